@@ -198,6 +198,40 @@ CUDANET_API int cudanet_k_attention_f8(const void* qkv, void* att, int B, int d,
 CUDANET_API int cudanet_k_layernorm_f8(int x_dtype, const void* x, const float* g, const float* b, void* h, int n,
                                        int d, int row_stride, float mul, void* stream, char* err, int err_len);
 
+/* The int8 linear layer with dynamic scales (no counterpart in the reference): rows of int8 codes q with one f32
+ * scale a row, q * scale standing for the row's values, and the product of two such matrices, whose scales are one
+ * for each row of A (token) and one for each row of W (output channel). No calibration: the scales are the rows' own.
+ *
+ * Device pointers on the current device, queued on `stream` (NULL: the legacy default stream), asynchronous: the call
+ * does not wait, allocates nothing and may be captured into a CUDA graph. Types: 0 = f16, 1 = bf16, 2 = f32. Rows have
+ * a pitch in elements (not used with a single row); what lies between a row's end and its pitch is neither read into
+ * a result nor written. M = 0 does nothing. Return 0, or -1 with the reason in err.
+ *
+ * A row's codes are q[i] = rint(t[i] * (127 / a)) (ties to even), a = max |t[i]|, so that -127 <= q <= 127. A row
+ * with a < 2^-120 has scale 0 and codes 0. A row that holds a NaN or an infinity (for the norm: or whose sum of
+ * squares leaves f32) has scale NaN and codes 0, so every product of it is NaN. */
+
+/* out = x + delta rounded to x's type (delta of x's type, or of any type where x is f32; out may be x or, of the same
+ * type, delta); then the codes of t = out * g and scale = a / sqrt(mean(out^2) + eps) / 127: q * scale stands for
+ * RMSNorm(out) * g. delta NULL: out must be NULL too, and the norm is of x. 1 <= D <= 32,768, eps > 0. */
+CUDANET_API int cudanet_k_rmsnorm_i8(int x_type, int delta_type, const void* x, const void* delta, const float* g,
+                                     void* out, void* q, float* scale, int M, int D, int64_t ldx, int64_t ldd,
+                                     int64_t ldo, int64_t ldq, float eps, void* stream, char* err, int err_len);
+
+/* The codes of x's rows and scale = a / 127. 1 <= D <= 32,768. The operand of cudanet_k_gemm_i8 from a product's
+ * output, and a weight matrix [N, K] with a scale for each output channel. */
+CUDANET_API int cudanet_k_quant_i8(int x_type, const void* x, void* q, float* scale, int M, int D, int64_t ldx,
+                                   int64_t ldq, void* stream, char* err, int err_len);
+
+/* C = epilogue(A[M, K] * W[N, K]^T): v = acc * rowscale[m] * colscale[n] + bias[n] (bias NULL: none), acc the exact
+ * int32 sum (any int8 codes, -128 included; 1 <= K <= 131,071, the largest K whose sums fit), with epi as for
+ * cudanet_k_gemm: 0: C 16-bit (`dtype`) = v; 1: C 16-bit = gelu(v); 2: C f32 += v; 3: C f32 = v. A and W begin on 16
+ * bytes and their row pitches are multiples of 16; C, bias and the scales may begin anywhere and C have any pitch
+ * >= N. kernel -1 chooses. Every kernel gives the same bits. */
+CUDANET_API int cudanet_k_gemm_i8(int dtype, int epi, int kernel, const void* A, const void* W, const float* rowscale,
+                                  const float* colscale, const float* bias, void* C, int M, int N, int K, int64_t lda,
+                                  int64_t ldw, int64_t ldc, void* stream, char* err, int err_len);
+
 #ifdef __cplusplus
 }
 #endif

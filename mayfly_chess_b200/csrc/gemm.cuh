@@ -238,8 +238,17 @@ struct GeluK {
     }
 };
 
-// s * gelu of both lanes of x2 (SCALED: s != 1)
-template <bool SCALED = false>
+// max(x, 0), NaN for a NaN
+__device__ __forceinline__ float relu_nan(float x)
+{
+    float y;
+    asm("max.NaN.f32 %0, %1, 0f00000000;" : "=f"(y) : "f"(x));
+    return y;
+}
+
+// s * gelu of both lanes of x2 (SCALED: s != 1). A NaN gives 0 unless KEEP_NAN, which costs nothing: the clamps drop
+// it, and relu(x) then carries it.
+template <bool SCALED = false, bool KEEP_NAN = false>
 __device__ __forceinline__ float2 gelu_pair(uint64_t x2, const GeluK& K)
 {
     const float2 x = upk2(x2);
@@ -257,6 +266,7 @@ __device__ __forceinline__ float2 gelu_pair(uint64_t x2, const GeluK& K)
     const uint64_t sq = pk2(ex2_approx_f(lp.x), ex2_approx_f(lp.y));      // s q
     float2 xs = x;
     if constexpr (SCALED) xs = upk2(mul2(x2, K.s));
+    if constexpr (KEEP_NAN) return upk2(fma2(na, sq, pk2(relu_nan(xs.x), relu_nan(xs.y))));
     return upk2(fma2(na, sq, pk2(fmaxf(xs.x, 0.f), fmaxf(xs.y, 0.f))));  // s relu(x) - s a q
 }
 

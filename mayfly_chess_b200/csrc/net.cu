@@ -32,6 +32,7 @@
 #include "attention_tc.cuh"
 #include "encode.cuh"
 #include "gemm_ln.cuh"
+#include "int8.cuh"
 #include "json_min.h"
 #include "trunk.cuh"
 
@@ -1647,6 +1648,66 @@ static void attention_once(const void* qkv, void* att, int B, int d, int heads, 
     if (e) throw std::runtime_error(std::string(who) + ": device error: " + err_site_name(e >> 8));
 }
 
+
+// ------------------------------------------------------------------------------------------------ int8 operators
+// The element types of the int8 entry points: the codes of the 16-bit kernels, and 2 = f32.
+enum I8Type : int { kI8F16 = 0, kI8BF16 = 1, kI8F32 = 2 };
+constexpr int kI8MaxRow = 32768;    // the longest row of the norm and the quantiser
+constexpr int kI8MaxK = 131071;     // 131,071 products of -128 * -128 are the most that an int32 sum holds
+
+static long long i8_bytes(int type) { return type == kI8F32 ? 4 : 2; }
+
+template <bool NORM, typename XT, typename DT>
+static void launch_rows_i8_t(const void* x, const void* delta, const float* g, void* out, void* q, float* scale,
+                             int M, int D, long long ldx, long long ldd, long long ldo, long long ldq, float eps,
+                             cudaStream_t s)
+{
+    launch_k(rows_i8_kernel<XT, DT, NORM>, dim3(static_cast<unsigned>(M)), dim3(256), 0, s, static_cast<const XT*>(x),
+             static_cast<const DT*>(delta), g, static_cast<XT*>(out), static_cast<int8_t*>(q), scale, D, ldx, ldd,
+             ldo, ldq, eps);
+}
+
+// k_rmsnorm_i8 (NORM) and k_quant_i8: x and delta of the types that the entry points take.
+template <bool NORM>
+static void launch_rows_i8(int x_type, int delta_type, const void* x, const void* delta, const float* g, void* out,
+                           void* q, float* scale, int M, int D, long long ldx, long long ldd, long long ldo,
+                           long long ldq, float eps, cudaStream_t s)
+{
+    auto go = [&](auto xt, auto dt) {
+        launch_rows_i8_t<NORM, decltype(xt), decltype(dt)>(x, delta, g, out, q, scale, M, D, ldx, ldd, ldo, ldq, eps, s);
+    };
+    if (x_type == kI8F16) go(__half(), __half());
+    else if (x_type == kI8BF16) go(__nv_bfloat16(), __nv_bfloat16());
+    else if (!NORM || delta_type == kI8F32) go(float(), float());
+    else if (delta_type == kI8F16) go(float(), __half());
+    else go(float(), __nv_bfloat16());
+}
+
+template <typename TO, int EPI>
+static void launch_gemm_i8_t(const void* A, const void* W, const float* rowscale, const float* colscale,
+                             const float* bias, void* C, int M, int N, int K, long long lda, long long ldw,
+                             long long ldc, cudaStream_t s)
+{
+    launch_k(gemm_i8_simple_kernel<TO, EPI>, dim3((N + 15) / 16, (M + 15) / 16), dim3(256), 0, s,
+             static_cast<const int8_t*>(A), static_cast<const int8_t*>(W), rowscale, colscale, bias,
+             static_cast<TO*>(C), M, N, K, lda, ldw, ldc);
+}
+
+// A null pointer, or one whose address is no multiple of `align`, named in the reason.
+static void need_ptr(const char* who, const char* name, const void* p, uintptr_t align)
+{
+    if (!p) throw std::runtime_error(std::string(who) + ": " + name + " is a null pointer");
+    if (reinterpret_cast<uintptr_t>(p) % align)
+        throw std::runtime_error(std::string(who) + ": " + name + " is not aligned to " + std::to_string(align) +
+                                 " bytes");
+}
+
+// A row pitch (elements) that is shorter than its row; the pitch of a single row is not used.
+static void need_pitch(const char* who, const char* name, long long ld, int width, int rows)
+{
+    if (rows > 1 && ld < width) throw std::runtime_error(std::string(who) + ": " + name + " is less than a row");
+}
+
 }  // namespace mf
 
 using mf::Net;
@@ -2145,6 +2206,101 @@ CUDANET_API int cudanet_k_layernorm_f8(int x_dtype, const void* x, const float* 
         else
             throw std::runtime_error("cudanet_k_layernorm_f8: x_dtype must be 0 (f32) or 1 (bf16)");
         mf::RT(cudaStreamSynchronize(s));
+        return 0;
+    });
+}
+
+// ------------------------------------------------------------------------------------------------ int8 operators
+CUDANET_API int cudanet_k_rmsnorm_i8(int x_type, int delta_type, const void* x, const void* delta, const float* g,
+                                     void* out, void* q, float* scale, int M, int D, int64_t ldx, int64_t ldd,
+                                     int64_t ldo, int64_t ldq, float eps, void* stream, char* err, int err_len)
+{
+    return mf::guarded(err, err_len, "cudanet_k_rmsnorm_i8: unknown exception", [&] {
+        const char* who = "cudanet_k_rmsnorm_i8";
+        if (x_type < mf::kI8F16 || x_type > mf::kI8F32 || delta_type < mf::kI8F16 || delta_type > mf::kI8F32)
+            throw std::runtime_error(std::string(who) + ": a type must be 0 (f16), 1 (bf16) or 2 (f32)");
+        if (delta && x_type != mf::kI8F32 && delta_type != x_type)
+            throw std::runtime_error(std::string(who) + ": delta must be of x's type, or x f32");
+        if (M < 0 || D < 1 || D > mf::kI8MaxRow)
+            throw std::runtime_error(std::string(who) + ": bad sizes (rows >= 0, 1 <= D <= 32768)");
+        if (!(eps > 0.f) || !std::isfinite(eps)) throw std::runtime_error(std::string(who) + ": eps must be positive");
+        if (M == 0) return 0;
+        const uintptr_t xb = static_cast<uintptr_t>(mf::i8_bytes(x_type));
+        mf::need_ptr(who, "x", x, xb);
+        mf::need_ptr(who, "g", g, 4);
+        mf::need_ptr(who, "q", q, 1);
+        mf::need_ptr(who, "scale", scale, 4);
+        mf::need_pitch(who, "ldx", ldx, D, M);
+        mf::need_pitch(who, "ldq", ldq, D, M);
+        if (delta) {
+            mf::need_ptr(who, "delta", delta, static_cast<uintptr_t>(mf::i8_bytes(delta_type)));
+            mf::need_ptr(who, "out", out, xb);
+            mf::need_pitch(who, "ldd", ldd, D, M);
+            mf::need_pitch(who, "ldo", ldo, D, M);
+        } else if (out) {
+            throw std::runtime_error(std::string(who) + ": out without delta: there is no sum to store");
+        }
+        mf::launch_rows_i8<true>(x_type, delta ? delta_type : x_type, x, delta, g, out, q, scale, M, D, ldx, ldd, ldo,
+                                 ldq, eps, static_cast<cudaStream_t>(stream));
+        return 0;
+    });
+}
+
+CUDANET_API int cudanet_k_quant_i8(int x_type, const void* x, void* q, float* scale, int M, int D, int64_t ldx,
+                                   int64_t ldq, void* stream, char* err, int err_len)
+{
+    return mf::guarded(err, err_len, "cudanet_k_quant_i8: unknown exception", [&] {
+        const char* who = "cudanet_k_quant_i8";
+        if (x_type < mf::kI8F16 || x_type > mf::kI8F32)
+            throw std::runtime_error(std::string(who) + ": x_type must be 0 (f16), 1 (bf16) or 2 (f32)");
+        if (M < 0 || D < 1 || D > mf::kI8MaxRow)
+            throw std::runtime_error(std::string(who) + ": bad sizes (rows >= 0, 1 <= D <= 32768)");
+        if (M == 0) return 0;
+        mf::need_ptr(who, "x", x, static_cast<uintptr_t>(mf::i8_bytes(x_type)));
+        mf::need_ptr(who, "q", q, 1);
+        mf::need_ptr(who, "scale", scale, 4);
+        mf::need_pitch(who, "ldx", ldx, D, M);
+        mf::need_pitch(who, "ldq", ldq, D, M);
+        mf::launch_rows_i8<false>(x_type, x_type, x, nullptr, nullptr, nullptr, q, scale, M, D, ldx, 0, 0, ldq, 0.f,
+                                  static_cast<cudaStream_t>(stream));
+        return 0;
+    });
+}
+
+CUDANET_API int cudanet_k_gemm_i8(int dtype, int epi, int kernel, const void* A, const void* W, const float* rowscale,
+                                  const float* colscale, const float* bias, void* C, int M, int N, int K, int64_t lda,
+                                  int64_t ldw, int64_t ldc, void* stream, char* err, int err_len)
+{
+    return mf::guarded(err, err_len, "cudanet_k_gemm_i8: unknown exception", [&] {
+        const char* who = "cudanet_k_gemm_i8";
+        if (dtype != 0 && dtype != 1) throw std::runtime_error(std::string(who) + ": dtype must be 0 (f16) or 1 (bf16)");
+        if (epi < 0 || epi > 3) throw std::runtime_error(std::string(who) + ": epi must be 0..3");
+        if (kernel != -1) throw std::runtime_error(std::string(who) + ": kernel must be -1");
+        if (M < 0 || N < 1 || K < 1 || K > mf::kI8MaxK)
+            throw std::runtime_error(std::string(who) + ": bad sizes (M >= 0, N >= 1, 1 <= K <= 131071)");
+        if (M == 0) return 0;
+        mf::need_ptr(who, "A", A, 16);
+        mf::need_ptr(who, "W", W, 16);
+        mf::need_ptr(who, "rowscale", rowscale, 4);
+        mf::need_ptr(who, "colscale", colscale, 4);
+        if (bias) mf::need_ptr(who, "bias", bias, 4);
+        mf::need_ptr(who, "C", C, epi >= 2 ? 4 : 2);
+        mf::need_pitch(who, "lda", lda, K, M);
+        mf::need_pitch(who, "ldw", ldw, K, N);
+        mf::need_pitch(who, "ldc", ldc, N, M);
+        if ((M > 1 && lda % 16) || (N > 1 && ldw % 16))
+            throw std::runtime_error(std::string(who) + ": the row pitches of A and W must be multiples of 16 bytes");
+        const cudaStream_t s = static_cast<cudaStream_t>(stream);
+        auto go = [&](auto to, auto e) {
+            mf::launch_gemm_i8_t<decltype(to), decltype(e)::value>(A, W, rowscale, colscale, bias, C, M, N, K, lda,
+                                                                   ldw, ldc, s);
+        };
+        using E0 = std::integral_constant<int, mf::kEpiBias>;
+        using E1 = std::integral_constant<int, mf::kEpiBiasGelu>;
+        if (epi == mf::kEpiResidual) go(float(), std::integral_constant<int, mf::kEpiResidual>());
+        else if (epi == mf::kEpiF32) go(float(), std::integral_constant<int, mf::kEpiF32>());
+        else if (dtype == 1) epi == 0 ? go(__nv_bfloat16(), E0()) : go(__nv_bfloat16(), E1());
+        else epi == 0 ? go(__half(), E0()) : go(__half(), E1());
         return 0;
     });
 }

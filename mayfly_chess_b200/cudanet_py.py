@@ -110,6 +110,15 @@ def load(dll=None):
         lib.cudanet_begin_keys.restype = i32
         lib.cudanet_encode_keys.argtypes = [vp, vp, vp, i32, vp, vp, vp, vp, vp, cp, i32]
         lib.cudanet_encode_keys.restype = i32
+        i64 = ctypes.c_int64
+        lib.cudanet_k_rmsnorm_i8.argtypes = [i32, i32, vp, vp, vp, vp, vp, vp, i32, i32, i64, i64, i64, i64, f32, vp,
+                                             cp, i32]
+        lib.cudanet_k_rmsnorm_i8.restype = i32
+        lib.cudanet_k_quant_i8.argtypes = [i32, vp, vp, vp, i32, i32, i64, i64, vp, cp, i32]
+        lib.cudanet_k_quant_i8.restype = i32
+        lib.cudanet_k_gemm_i8.argtypes = [i32, i32, i32, vp, vp, vp, vp, vp, vp, i32, i32, i32, i64, i64, i64, vp, cp,
+                                          i32]
+        lib.cudanet_k_gemm_i8.restype = i32
         _libs[path] = lib
         return lib
 
@@ -571,3 +580,142 @@ def k_layernorm_f8(x, g, b, h, n, d, mul, row_stride=1, dll=None):
     if rc != 0:
         raise RuntimeError(f"cudanet_k_layernorm_f8: {_msg(err)}")
     return h
+
+
+# ------------------------------------------------------------------------------------------------ int8 operators
+# These calls queue one kernel and return, so what a call costs on the host is most of what a small one costs: the
+# checks read each tensor's attributes once, and the reason buffer is kept per thread.
+_i8_local = threading.local()
+_i8_types = {}
+
+
+def _i8_reason():
+    try:
+        return _i8_local.reason
+    except AttributeError:
+        _i8_local.reason = ctypes.create_string_buffer(ERR_LEN)
+        return _i8_local.reason
+
+
+def _i8_type(t, name):
+    """The C ABI's code of a tensor's element type: 0 f16, 1 bf16, 2 f32."""
+    if not _i8_types:
+        import torch
+        _i8_types.update({torch.float16: 0, torch.bfloat16: 1, torch.float32: 2})
+    code = _i8_types.get(t.dtype)
+    if code is None:
+        raise ValueError(f"{name}: float16, bfloat16 or float32 only, got {t.dtype}")
+    return code
+
+
+def _i8_codes(t, name):
+    import torch
+    if t.dtype != torch.int8:
+        raise ValueError(f"{name}: int8 only, got {t.dtype}")
+
+
+def _i8_vec(t, name, n, dev):
+    """A contiguous float32 vector of n elements on device index dev; its address."""
+    if _i8_type(t, name) != 2:
+        raise ValueError(f"{name}: float32 only, got {t.dtype}")
+    if t.shape != (n,) or (n > 1 and t.stride(0) != 1):
+        raise ValueError(f"{name}: shape {tuple(t.shape)} strides {t.stride()}, expected ({n},) contiguous")
+    if t.get_device() != dev:
+        raise ValueError(f"{name}: on {t.device}, expected cuda:{dev}")
+    return t.data_ptr()
+
+
+def _i8_mat(t, name, shape, dev):
+    """The row pitch of a matrix whose rows are contiguous, after the checks of its shape and device."""
+    if t.shape != shape:
+        raise ValueError(f"{name}: shape {tuple(t.shape)}, expected {tuple(shape)}")
+    if t.get_device() != dev:
+        raise ValueError(f"{name}: on {t.device}, expected cuda:{dev}")
+    pitch, step = t.stride()
+    if step != 1 and shape[1] > 1:
+        raise ValueError(f"{name}: rows must be contiguous, got strides {t.stride()}")
+    return pitch
+
+
+def _i8_device(t, name):
+    """The index of the CUDA device a 2-d tensor is on."""
+    if t.dim() != 2:
+        raise ValueError(f"{name}: shape {tuple(t.shape)}, expected a matrix")
+    dev = t.get_device()
+    if dev < 0:
+        raise ValueError(f"{name}: needs a CUDA tensor, got one on {t.device}")
+    return dev
+
+
+def _i8_call(fn, dev, *args):
+    """fn(*args, stream, reason) on device `dev` and its current stream; RuntimeError with the library's reason."""
+    import torch
+    if torch.cuda.current_device() != dev:
+        with torch.cuda.device(dev):
+            return _i8_call(fn, dev, *args)
+    reason = _i8_reason()
+    if fn(*args, torch.cuda.current_stream(dev).cuda_stream, reason, ERR_LEN) != 0:
+        raise RuntimeError(f"{fn.__name__}: {_msg(reason)}")
+
+
+def k_rmsnorm_i8(x, delta, g, out, q, scale, eps=1e-6, dll=None):
+    """out = x + delta in x's type, and its RMS norm times g as int8 rows with a float32 scale each: q * scale stands
+    for out / sqrt(mean(out^2) + eps) * g. x (M, D) float32, bfloat16 or float16; delta the same shape, of x's type or
+    of any of the three where x is float32; out may be x (in place). delta and out None: the norm of x alone. q (M, D)
+    int8, scale (M,) float32. Rows may have any pitch; asynchronous on the device's current stream. Returns (q,
+    scale)."""
+    lib = load(dll)
+    dev = _i8_device(x, "x")
+    shape = x.shape
+    M, D = shape
+    xt = _i8_type(x, "x")
+    ldx, ldq = _i8_mat(x, "x", shape, dev), _i8_mat(q, "q", shape, dev)
+    _i8_codes(q, "q")
+    gp, sp = _i8_vec(g, "g", D, dev), _i8_vec(scale, "scale", M, dev)
+    if (delta is None) != (out is None):
+        raise ValueError("delta and out: both or neither (out holds the sum)")
+    if delta is None:
+        dt, ldd, ldo, dp, op = xt, 0, 0, None, None
+    else:
+        dt, ldd, ldo = _i8_type(delta, "delta"), _i8_mat(delta, "delta", shape, dev), _i8_mat(out, "out", shape, dev)
+        if out.dtype != x.dtype:
+            raise ValueError(f"out: {x.dtype} as x, got {out.dtype}")
+        dp, op = delta.data_ptr(), out.data_ptr()
+    _i8_call(lib.cudanet_k_rmsnorm_i8, dev, xt, dt, x.data_ptr(), dp, gp, op, q.data_ptr(), sp, M, D, ldx, ldd, ldo,
+             ldq, eps)
+    return q, scale
+
+
+def k_quant_i8(x, q, scale, dll=None):
+    """x (M, D) float32, bfloat16 or float16 as int8 rows with a float32 scale each: scale = max |row| / 127, q * scale
+    stands for x. A weight matrix (N, K) gets a scale for each output channel. Rows may have any pitch; asynchronous on
+    the device's current stream. Returns (q, scale)."""
+    lib = load(dll)
+    dev = _i8_device(x, "x")
+    shape = x.shape
+    M, D = shape
+    ldx, ldq = _i8_mat(x, "x", shape, dev), _i8_mat(q, "q", shape, dev)
+    _i8_codes(q, "q")
+    _i8_call(lib.cudanet_k_quant_i8, dev, _i8_type(x, "x"), x.data_ptr(), q.data_ptr(), _i8_vec(scale, "scale", M, dev),
+             M, D, ldx, ldq)
+    return q, scale
+
+
+def k_gemm_i8(A, W, rowscale, colscale, bias, C, epi, kernel=-1, dll=None):
+    """C = epilogue(A W^T * rowscale[m] * colscale[n] + bias[n]) with int8 A (M, K) and W (N, K), whose rows begin on
+    16 bytes, the sum exact in int32, rowscale (M,), colscale (N,) and bias (N,) or None float32: epi 0 16-bit out, 1
+    GELU and 16-bit out, 2 C += (float32), 3 float32 out. Asynchronous on the device's current stream. Returns C."""
+    lib = load(dll)
+    dev = _i8_device(A, "A")
+    _i8_codes(A, "A")
+    _i8_codes(W, "W")
+    M, K = A.shape
+    N = W.shape[0]
+    lda, ldw, ldc = _i8_mat(A, "A", (M, K), dev), _i8_mat(W, "W", (N, K), dev), _i8_mat(C, "C", (M, N), dev)
+    ct = _i8_type(C, "C")
+    if (ct == 2) != (epi >= 2):
+        raise ValueError(f"C: epi {epi} writes {'float32' if epi >= 2 else '16-bit floats'}, got {C.dtype}")
+    _i8_call(lib.cudanet_k_gemm_i8, dev, ct & 1, epi, kernel, A.data_ptr(), W.data_ptr(),
+             _i8_vec(rowscale, "rowscale", M, dev), _i8_vec(colscale, "colscale", N, dev),
+             None if bias is None else _i8_vec(bias, "bias", N, dev), C.data_ptr(), M, N, K, lda, ldw, ldc)
+    return C

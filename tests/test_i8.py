@@ -1,0 +1,89 @@
+"""What the int8 entry points refuse on the host, through the C ABI: no GPU, nothing is queued."""
+import ctypes
+
+import pytest
+
+P = 1 << 20          # an address that no refused call looks at
+
+
+@pytest.fixture(scope="module")
+def lib():
+    from mayfly_chess_b200 import build, cudanet_py
+    build.build()
+    return cudanet_py.load()
+
+
+def refused(fn, args, names, reason, **change):
+    values = dict(zip(names, args))
+    for n in change:
+        assert n in values
+    values.update(change)
+    err = ctypes.create_string_buffer(512)
+    assert fn(*values.values(), None, err, 512) == -1
+    assert reason in err.value.decode(), err.value
+
+
+GEMM = ("dtype", "epi", "kernel", "A", "W", "rowscale", "colscale", "bias", "C", "M", "N", "K", "lda", "ldw", "ldc")
+
+
+@pytest.mark.parametrize("reason,change", [
+    ("dtype", {"dtype": 2}), ("dtype", {"dtype": -1}), ("epi", {"epi": 4}), ("epi", {"epi": -1}),
+    ("kernel", {"kernel": 77}), ("bad sizes", {"M": -1}), ("bad sizes", {"N": 0}), ("bad sizes", {"K": 0}),
+    ("bad sizes", {"K": 131072}), ("A is a null", {"A": None}), ("W is a null", {"W": None}),
+    ("rowscale is a null", {"rowscale": None}), ("colscale is a null", {"colscale": None}), ("C is a null", {"C": None}),
+    ("A is not aligned to 16", {"A": P + 8}), ("W is not aligned to 16", {"W": P + 1}),
+    ("rowscale is not aligned to 4", {"rowscale": P + 2}), ("bias is not aligned to 4", {"bias": P + 1}),
+    ("C is not aligned to 2", {"C": P + 1}), ("C is not aligned to 4", {"C": P + 2, "epi": 3}),
+    ("lda is less", {"lda": 48}), ("ldw is less", {"ldw": 0}), ("ldc is less", {"ldc": 31}),
+    ("multiples of 16", {"lda": 72}), ("multiples of 16", {"ldw": 65})])
+def test_gemm_refusals(lib, reason, change):
+    args = (1, 0, -1, P, P, P, P, P, P, 5, 32, 64, 64, 64, 32)
+    refused(lib.cudanet_k_gemm_i8, args, GEMM, reason, **change)
+
+
+NORM = ("x_type", "delta_type", "x", "delta", "g", "out", "q", "scale", "M", "D", "ldx", "ldd", "ldo", "ldq", "eps")
+
+
+@pytest.mark.parametrize("reason,change", [
+    ("type", {"x_type": 3}), ("type", {"delta_type": -1}), ("x's type", {"x_type": 1, "delta_type": 0}),
+    ("x's type", {"x_type": 0, "delta_type": 2}), ("bad sizes", {"M": -3}), ("bad sizes", {"D": 0}),
+    ("bad sizes", {"D": 32769}), ("eps", {"eps": 0.0}), ("eps", {"eps": float("nan")}), ("eps", {"eps": float("inf")}),
+    ("x is a null", {"x": None}), ("g is a null", {"g": None}), ("q is a null", {"q": None}),
+    ("scale is a null", {"scale": None}), ("out is a null", {"out": None}), ("out without delta", {"delta": None}),
+    ("x is not aligned", {"x": P + 2}), ("delta is not aligned", {"delta": P + 1}), ("out is not aligned", {"out": P + 2}),
+    ("ldx is less", {"ldx": 63}), ("ldd is less", {"ldd": 1}), ("ldo is less", {"ldo": -64}), ("ldq is less", {"ldq": 0})])
+def test_rmsnorm_refusals(lib, reason, change):
+    args = (2, 1, P, P, P, P, P, P, 5, 64, 64, 64, 64, 64, 1e-6)
+    refused(lib.cudanet_k_rmsnorm_i8, args, NORM, reason, **change)
+
+
+QUANT = ("x_type", "x", "q", "scale", "M", "D", "ldx", "ldq")
+
+
+@pytest.mark.parametrize("reason,change", [
+    ("x_type", {"x_type": 3}), ("bad sizes", {"M": -1}), ("bad sizes", {"D": 0}), ("bad sizes", {"D": 32769}),
+    ("x is a null", {"x": None}), ("q is a null", {"q": None}), ("scale is a null", {"scale": None}),
+    ("x is not aligned", {"x": P + 1}), ("scale is not aligned", {"scale": P + 2}), ("ldx is less", {"ldx": 63}),
+    ("ldq is less", {"ldq": 0})])
+def test_quant_refusals(lib, reason, change):
+    refused(lib.cudanet_k_quant_i8, (0, P, P, P, 5, 64, 64, 64), QUANT, reason, **change)
+
+
+def test_no_rows_is_nothing_to_do(lib):
+    err = ctypes.create_string_buffer(64)
+    assert lib.cudanet_k_quant_i8(0, None, None, None, 0, 64, 0, 0, None, err, 64) == 0
+    assert lib.cudanet_k_rmsnorm_i8(0, 0, None, None, None, None, None, None, 0, 64, 0, 0, 0, 0, 1e-6, None, err, 64) == 0
+    assert lib.cudanet_k_gemm_i8(0, 0, -1, None, None, None, None, None, None, 0, 8, 64, 0, 0, 0, None, err, 64) == 0
+
+
+def test_wrappers_refuse_host_tensors():
+    import torch
+
+    from mayfly_chess_b200 import cudanet_py as k
+    x, q, s = torch.ones(2, 16), torch.ones(2, 16, dtype=torch.int8), torch.ones(2)
+    with pytest.raises(ValueError, match="CUDA"):
+        k.k_quant_i8(x, q, s)
+    with pytest.raises(ValueError, match="CUDA"):
+        k.k_rmsnorm_i8(x, x, torch.ones(16), x, q, s)
+    with pytest.raises(ValueError, match="CUDA"):
+        k.k_gemm_i8(q, q, s, s, None, torch.empty(2, 2), 3)

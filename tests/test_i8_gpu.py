@@ -1,0 +1,433 @@
+"""The int8 linear layer (k_rmsnorm_i8, k_quant_i8, k_gemm_i8) on a B200 against its definition in 64 bits.
+
+Tolerances count the roundings between the definition and the result, u = 2^-24 each (half a step of f32, relative):
+  codes    t * (127 / a) has a rounding in the factor and one in the product (for the norm one in t = s * g and one in
+           a too), and is at most 127: off by 127 * 4u at most before it is rounded to a whole number, so a code is
+           within 0.5 + 127 * 4u of the exact quotient
+  scale    quantiser: one division, exactly the f32 quotient. Norm: a sum of squares of D terms, each thread at most
+           D / 32 of them one after another and then a tree of at most 10 adds, each rounding at most u; the square
+           root halves that; rsqrtf is within 2 steps (4u), and the mean, eps, t, a * r and the quotient are 5 more
+  product  acc is exact; its conversion, two scalings and the bias are 4 roundings: 2u of |acc rs cs| and u of the
+           result, and twice that bounds them; the 16-bit output adds eps / 2 of its type, GELU the 2.5e-5 of
+           a * Phi(-a) (at most 0.17) of its polynomial and its slope of at most 1.13
+"""
+import math
+
+import pytest
+import torch
+
+pytestmark = pytest.mark.gpu
+
+U = 2.0 ** -24
+DT = {"f32": torch.float32, "bf16": torch.bfloat16, "f16": torch.float16}
+
+
+@pytest.fixture(scope="module")
+def k():
+    from mayfly_chess_b200 import build, cudanet_py
+    build.build()
+    if not torch.cuda.is_available():
+        pytest.skip("no CUDA device")
+    return cudanet_py
+
+
+def gen(seed):
+    return torch.Generator(device="cuda").manual_seed(seed)
+
+
+def matrix(rows, cols, dtype, pitch=None, fill=0, offset=0):
+    """A (rows, cols) view, `offset` elements into a buffer of rows of `pitch` that is filled with `fill`; and the
+    buffer."""
+    pitch = cols if pitch is None else pitch
+    full = torch.full((rows * pitch + offset,), fill, dtype=dtype, device="cuda")
+    return full[offset:].view(rows, pitch)[:, :cols], full
+
+
+def untouched(view, full, fill, offset=0):
+    """Whether nothing outside the view was written."""
+    keep = full.clone()
+    rows, cols = view.shape
+    keep[offset:].view(rows, -1)[:, :cols] = fill
+    want = torch.full_like(full, fill)
+    return torch.equal(keep.view(torch.uint8), want.view(torch.uint8))
+
+
+def row_scale(x):
+    """max |row| / 127 in f32: the quotient in 64 bits (of two tensors: torch multiplies by a number's reciprocal),
+    which has more than twice f32's bits, rounded once."""
+    a = x.double().abs().amax(1)
+    return (a / torch.full_like(a, 127)).float()
+
+
+def check_codes(q, scale, t64, scale64, scale_tol):
+    """q and scale against the exact t (up to a row factor) and scale; every row here has something to scale."""
+    a = t64.abs().amax(1, keepdim=True)
+    assert ((scale.double() - scale64).abs() <= scale_tol * scale64).all()
+    assert ((q.double() - 127 * t64 / a).abs() <= 0.5 + 127 * 4 * U).all()
+    assert (q.abs().amax(1) == 127).all()
+
+
+# ------------------------------------------------------------------------------------------------ rows
+SHAPES = [(1, 1), (1, 1024), (3, 7), (5, 8), (2, 31), (65, 256), (66, 997), (7, 1000), (33, 1024), (4, 2048), (3, 4104),
+          (2, 8191), (5, 8192), (2, 20001), (1, 32768), (3, 32760), (1300, 1024), (600, 72)]
+
+
+@pytest.mark.parametrize("M,D", SHAPES)
+@pytest.mark.parametrize("x", ["f32", "bf16", "f16"])
+def test_quant(k, M, D, x):
+    g = gen(M * 31 + D)
+    X = (torch.randn(M, D, device="cuda", generator=g) * 3).to(DT[x])
+    X[:, 0] = 1.0                      # no row of zeros
+    q, scale = torch.empty(M, D, dtype=torch.int8, device="cuda"), torch.empty(M, device="cuda")
+    assert k.k_quant_i8(X, q, scale) == (q, scale)
+    t = X.double()
+    assert torch.equal(scale, row_scale(X))
+    check_codes(q, scale, t, t.abs().amax(1) / 127, U)
+
+
+@pytest.mark.parametrize("M,D", SHAPES)
+@pytest.mark.parametrize("x,delta", [("f32", "f32"), ("f32", "bf16"), ("f32", "f16"), ("f32", None), ("bf16", "bf16"),
+                                     ("bf16", None), ("f16", "f16"), ("f16", None)])
+def test_rmsnorm(k, M, D, x, delta):
+    r = gen(M * 37 + D)
+    X = torch.randn(M, D, device="cuda", generator=r).to(DT[x])
+    X[:, 0] = 4.0
+    G = 1 + 0.1 * torch.randn(D, device="cuda", generator=r)
+    Dl = torch.randn(M, D, device="cuda", generator=r).to(DT[delta]) if delta else None
+    want = X if delta is None else (X.float() + Dl.float()).to(X.dtype)
+    out = torch.empty_like(X) if delta else None
+    X0 = X.clone()
+    q, scale = torch.empty(M, D, dtype=torch.int8, device="cuda"), torch.empty(M, device="cuda")
+    k.k_rmsnorm_i8(X, Dl, G, out, q, scale, 1e-5)
+    if delta:
+        assert torch.equal(out, want) and torch.equal(X, X0)
+    s = want.double()
+    t = s * G.double()
+    scale64 = t.abs().amax(1) / torch.sqrt(s.square().mean(1) + float(torch.tensor(1e-5))) / 127
+    check_codes(q, scale, t, scale64, ((D / 32 + 10) / 2 + 9) * U)
+    if delta:                          # in place, the same bits
+        q2, scale2 = torch.empty_like(q), torch.empty_like(scale)
+        k.k_rmsnorm_i8(X, Dl, G, X, q2, scale2, 1e-5)
+        assert torch.equal(X, want) and torch.equal(q2, q) and torch.equal(scale2, scale)
+
+
+@pytest.mark.parametrize("x", ["f32", "bf16", "f16"])
+@pytest.mark.parametrize("D,px,pd,po,pq,off", [(64, 64, 80, 72, 64, 0), (64, 65, 66, 67, 68, 1), (1000, 1008, 1000, 1001, 1008, 0),
+                                               (100, 112, 104, 108, 112, 3), (2048, 2056, 2049, 2048, 2064, 8)])
+def test_rows_of_any_pitch_and_start(k, x, D, px, pd, po, pq, off):
+    """Every pitch and start gives the bits of the contiguous call, and nothing outside the rows is written."""
+    M, r = 37, gen(D + px)
+    X0 = torch.randn(M, D, device="cuda", generator=r).to(DT[x])
+    D0 = torch.randn(M, D, device="cuda", generator=r).to(DT[x])
+    G = torch.randn(D + 1, device="cuda", generator=r)[1:]
+    want = [torch.empty_like(X0), torch.empty(M, D, dtype=torch.int8, device="cuda"), torch.empty(M, device="cuda")]
+    k.k_rmsnorm_i8(X0, D0, G, *want)
+    X, _ = matrix(M, D, DT[x], px, 9, off)
+    Dl, _ = matrix(M, D, DT[x], pd, 9, off)
+    out, fo = matrix(M, D, DT[x], po, 9, off)
+    q, fq = matrix(M, D, torch.int8, pq, 99, off)
+    scale = torch.full((M + 2,), 9.0, device="cuda")
+    X.copy_(X0)
+    Dl.copy_(D0)
+    k.k_rmsnorm_i8(X, Dl, G, out, q, scale[1:-1])
+    assert torch.equal(out, want[0]) and torch.equal(q, want[1])
+    # the sum of squares may be added in another order for rows that are read in another way
+    assert ((scale[1:-1] - want[2]).abs() <= (D / 32 + 10) * U * want[2]).all()
+    assert untouched(out, fo, 9, off) and untouched(q, fq, 99, off) and scale[0] == 9 and scale[-1] == 9
+    qq, fq = matrix(M, D, torch.int8, pq, 99, off)
+    k.k_quant_i8(X, qq, scale[1:-1])
+    assert torch.equal(scale[1:-1], row_scale(X0))
+    check_codes(qq, scale[1:-1], X0.double(), X0.double().abs().amax(1) / 127, U)
+    assert untouched(qq, fq, 99, off)
+
+
+@pytest.mark.parametrize("D", [1, 33, 1024, 9000])
+@pytest.mark.parametrize("x", ["f32", "bf16", "f16"])
+def test_rows_with_nothing_to_scale(k, D, x):
+    """Zero rows, rows of numbers too small to scale, and rows that hold a NaN or an infinity, among ordinary rows."""
+    inf, nan = math.inf, math.nan
+    X = torch.randn(10, D, device="cuda").to(DT[x])
+    X[:, 0] = 2.0
+    X[1] = 0.0
+    X[2, D // 2] = nan
+    X[3, D - 1] = inf
+    X[4, D // 3] = -inf
+    X[5] = -0.0
+    X[6, 0], X[6, D - 1] = inf, nan
+    if x != "f16":
+        X[7] = 1e-38
+    q, scale = torch.full((10, D), 99, dtype=torch.int8, device="cuda"), torch.full((10,), 9.0, device="cuda")
+    k.k_quant_i8(X, q, scale)
+    fine = [0, 8, 9] + ([7] if x == "f16" else [])
+    zero = [1, 5] + ([] if x == "f16" else [7])
+    assert torch.equal(scale[fine], row_scale(X[fine]))
+    assert (scale[zero] == 0).all() and (q[zero] == 0).all()
+    assert torch.isnan(scale[[2, 3, 4, 6]]).all() and (q[[2, 3, 4, 6]] == 0).all()
+    G = torch.ones(D, device="cuda")
+    q.fill_(99)
+    k.k_rmsnorm_i8(X, None, G, None, q, scale)
+    assert (scale[fine] > 0).all() and (q[fine].abs().amax(1) == 127).all()
+    assert (scale[zero] == 0).all() and (q[zero] == 0).all()
+    assert torch.isnan(scale[[2, 3, 4, 6]]).all() and (q[[2, 3, 4, 6]] == 0).all()
+    if x != "f16":                      # squares over f32
+        X.fill_(3e38)
+        k.k_rmsnorm_i8(X, None, G, None, q, scale)
+        assert torch.isnan(scale).all() and (q == 0).all()
+    G.zero_()                           # a norm whose weight is zero
+    k.k_rmsnorm_i8(X[:1].clone().fill_(1.0), None, G, None, q[:1], scale[:1])
+    assert scale[0] == 0 and (q[0] == 0).all()
+
+
+def test_codes_at_the_ties(k):
+    """A row whose largest is 127 has the factor 1: its codes are its values rounded to the nearest, ties to even."""
+    X = torch.arange(-127, 127.5, 0.5, device="cuda")[None].contiguous()
+    q, scale = torch.empty(X.shape, dtype=torch.int8, device="cuda"), torch.empty(1, device="cuda")
+    k.k_quant_i8(X, q, scale)
+    assert scale[0] == 1 and torch.equal(q.float(), torch.round(X))
+
+
+# ------------------------------------------------------------------------------------------------ product
+def operands(M, N, K, seed, full=False):
+    """Codes whose rows begin on 16 bytes, what lies behind them filled with codes that must not count."""
+    r = gen(seed)
+    pitch = (K + 15) // 16 * 16 + 16
+    A, _ = matrix(M, K, torch.int8, pitch, 77)
+    W, _ = matrix(N, K, torch.int8, pitch, -99)
+    for t in (A, W):
+        t.copy_(torch.randint(-128, 128, t.shape, device="cuda", generator=r, dtype=torch.int32).to(torch.int8))
+    rs = (torch.rand(M, device="cuda", generator=r) + 0.5) / 64
+    cs = (torch.rand(N, device="cuda", generator=r) + 0.5) / (64 * math.sqrt(K))
+    bias = torch.randn(N, device="cuda", generator=r) * 0.1
+    return A, W, rs, cs, bias
+
+
+def check_product(C, C0, A, W, rs, cs, bias, epi):
+    acc = A.double() @ W.double().t()                # whole numbers below 2^53: exact
+    p = acc * rs.double()[:, None] * cs.double()
+    v = p if bias is None else p + bias.double()
+    tol = 2 * (2 * U * p.abs() + U * v.abs())
+    if epi == 1:
+        v = v * torch.special.ndtr(v)
+        tol = 1.13 * tol + 2.5e-5 * 0.17 + 4 * U * v.abs()
+    if epi == 2:
+        v = v + C0.double()
+        tol = tol + U * v.abs()
+    if epi < 2:
+        f = torch.finfo(C.dtype)
+        tol = tol + (v.abs() + tol) * f.eps / 2 + f.smallest_normal * f.eps / 2
+    excess = ((C.double() - v).abs() - tol).max().item()
+    assert math.isfinite(excess) and excess <= 0, excess
+
+
+SIZES = [(1, 1, 1), (1, 8324, 1024), (2, 7, 15), (3, 64, 16), (5, 129, 130), (16, 1000, 2048), (17, 100, 31), (33, 257, 4100),
+         (65, 2048, 1024), (64, 128, 128), (129, 72, 1000), (128, 256, 64), (300, 1001, 200), (777, 512, 257),
+         (1040, 1024, 1024), (4160, 776, 384)]
+
+
+@pytest.mark.parametrize("M,N,K", SIZES)
+@pytest.mark.parametrize("epi,out", [(0, "bf16"), (0, "f16"), (1, "bf16"), (1, "f16"), (2, "f32"), (3, "f32")])
+def test_gemm(k, M, N, K, epi, out):
+    A, W, rs, cs, bias = operands(M, N, K, M * 7 + N + K + epi)
+    if N % 3 == 0:
+        bias = None
+    # rows padded to whole 16 bytes and to more, and rows that begin anywhere
+    first = None
+    for pitch, off in ((N, 0), ((N + 15) // 8 * 8, 0), (N + 3, 1)):
+        C, full = matrix(M, N, DT[out], pitch, 7, off)
+        if epi == 2:
+            C.copy_(torch.randn(M, N, device="cuda", generator=gen(N)))
+        C0 = C.clone()
+        assert k.k_gemm_i8(A, W, rs, cs, bias, C, epi) is C
+        check_product(C, C0, A, W, rs, cs, bias, epi)
+        assert untouched(C, full, 7, off)
+        first = C.clone() if first is None else first
+        assert torch.equal(C, first)
+
+
+@pytest.mark.parametrize("M", [1, 20, 300])
+def test_gemm_largest_sums(k, M):
+    """The longest K at the largest products: the int32 sum comes to 2^31 - 16,384."""
+    K = 131071
+    A, W, rs, cs, _ = operands(M, 40, K, 5)
+    A.fill_(-128)
+    W.fill_(-128)
+    W[1].fill_(127)
+    C = torch.empty(M, 40, device="cuda")
+    one = torch.ones(M, device="cuda"), torch.ones(40, device="cuda")
+    k.k_gemm_i8(A, W, *one, None, C, 3)
+    want = torch.full((M, 40), float(128 * 128 * K), device="cuda")
+    want[:, 1] = -128.0 * 127 * K
+    assert torch.equal(C, want)
+
+
+def test_gemm_nan_scale_marks_its_row(k):
+    A, W, rs, cs, bias = operands(70, 96, 64, 3)
+    rs[3] = math.nan
+    for out, epi in (("bf16", 0), ("f16", 1), ("f32", 2), ("f32", 3)):
+        C = torch.zeros(70, 96, dtype=DT[out], device="cuda")
+        k.k_gemm_i8(A, W, rs, cs, bias, C, epi)
+        bad = torch.isnan(C)
+        assert bad[3].all() and not bad[[i for i in range(70) if i != 3]].any()
+
+
+def test_gemm_offset_vectors(k):
+    """Scales and bias that begin on 4 bytes, and operands that are rows of larger matrices."""
+    A, W, rs, cs, bias = operands(400, 520, 256, 9)
+    want = torch.empty(390, 511, dtype=torch.bfloat16, device="cuda")
+    k.k_gemm_i8(A[10:], W[9:], rs[10:].clone(), cs[9:].clone(), bias[9:].clone(), want, 0)
+    got = torch.empty_like(want)
+    k.k_gemm_i8(A[10:], W[9:], rs[10:], cs[9:], bias[9:], got, 0)
+    assert torch.equal(got, want)
+    check_product(got, None, A[10:], W[9:], rs[10:], cs[9:], bias[9:], 0)
+
+
+def test_offsets_past_32_bits(k):
+    """Rows whose elements lie more than 2^31 elements into their buffers."""
+    M, D, pitch = 70000, 48, 32768
+    X = torch.empty(M, pitch, dtype=torch.float16, device="cuda")[:, :D]
+    X.copy_(torch.randn(M, D, device="cuda", generator=gen(1)))
+    q = torch.empty(M, pitch, dtype=torch.int8, device="cuda")[:, :D]
+    scale = torch.empty(M, device="cuda")
+    k.k_quant_i8(X, q, scale)
+    check_codes(q, scale, X.double(), X.double().abs().amax(1) / 127, U)
+    W = torch.randint(-127, 128, (40, D), device="cuda", dtype=torch.int32).to(torch.int8)
+    cs = torch.full((40,), 0.01, device="cuda")
+    for epi, p in ((0, pitch), (2, pitch), (0, pitch + 1)):
+        C = torch.zeros(M, p, dtype=torch.float32 if epi else torch.bfloat16, device="cuda")[:, :40]
+        k.k_gemm_i8(q, W, scale, cs, None, C, epi)
+        check_product(C, torch.zeros(M, 40, device="cuda"), q, W, scale, cs, None, epi)
+
+
+# ------------------------------------------------------------------------------------------------ together
+def block(k, b):
+    """A feed-forward block on int8 products: norm with the residual's addition, product + GELU, quantiser, product."""
+    k.k_rmsnorm_i8(b["x"], b["delta"], b["g"], b["out"], b["q"], b["s"])
+    k.k_gemm_i8(b["q"], b["W1"], b["s"], b["c1"], b["b1"], b["h"], 1)
+    k.k_quant_i8(b["h"], b["q2"], b["s2"])
+    k.k_gemm_i8(b["q2"], b["W2"], b["s2"], b["c2"], b["b2"], b["out"], 2)
+
+
+def block_state(k, M, d, ff, seed):
+    r = gen(seed)
+    e = lambda *n, dtype=torch.float32: torch.empty(*n, dtype=dtype, device="cuda")  # noqa: E731
+    b = {"x": torch.randn(M, d, device="cuda", generator=r), "g": 1 + 0.1 * torch.randn(d, device="cuda", generator=r),
+         "delta": torch.randn(M, d, device="cuda", generator=r).bfloat16(), "out": e(M, d),
+         "q": e(M, d, dtype=torch.int8), "s": e(M), "h": e(M, ff, dtype=torch.bfloat16),
+         "q2": e(M, ff, dtype=torch.int8), "s2": e(M), "b1": torch.randn(ff, device="cuda", generator=r) * 0.1,
+         "b2": torch.randn(d, device="cuda", generator=r) * 0.1,
+         "w1": torch.randn(ff, d, device="cuda", generator=r) / math.sqrt(d),
+         "w2": torch.randn(d, ff, device="cuda", generator=r) / math.sqrt(ff)}
+    for i, (n, kk) in ((1, (ff, d)), (2, (d, ff))):
+        b[f"W{i}"], b[f"c{i}"] = k.k_quant_i8(b[f"w{i}"], e(n, kk, dtype=torch.int8), e(n))
+    return b
+
+
+@pytest.mark.parametrize("M,d,ff", [(1, 256, 1024), (65, 1024, 2048), (520, 1008, 2000), (2080, 1024, 2048)])
+def test_block(k, M, d, ff):
+    b = block_state(k, M, d, ff, M)
+    block(k, b)
+    # each step against its definition on what the step before it stored
+    s = b["x"] + b["delta"].float()
+    t = s.double() * b["g"].double()
+    r64 = 1 / torch.sqrt(s.double().square().mean(1) + float(torch.tensor(1e-6)))
+    check_codes(b["q"], b["s"], t, t.abs().amax(1) * r64 / 127, ((d / 32 + 10) / 2 + 9) * U)
+    check_product(b["h"], None, b["q"], b["W1"], b["s"], b["c1"], b["b1"], 1)
+    h = b["h"].double()
+    check_codes(b["q2"], b["s2"], h, h.abs().amax(1) / 127, U)
+    check_product(b["out"], s, b["q2"], b["W2"], b["s2"], b["c2"], b["b2"], 2)
+    # and the whole against the block in 64 bits without quantising: a code is off by up to half a step of a row's
+    # largest / 127, uniformly, so by (largest / rms) / (127 sqrt 12) of the row's rms. With a largest of at most 5.5 rms
+    # (normal rows of up to 2,048) that is 1.25%; the GELU's rows have a largest of up to 8 rms: 1.8%. Four operands,
+    # independent: sqrt(3 * 1.25^2 + 1.8^2) < 2.9%, and GELU passes on at most 1.13 of its input's error: 3.3%
+    y = t * r64[:, None]
+    f = y @ b["w1"].double().t() + b["b1"].double()
+    f = (f * torch.special.ndtr(f)) @ b["w2"].double().t() + b["b2"].double()
+    got = b["out"].double() - s.double()
+    assert (got - f).norm() <= 0.033 * f.norm()
+
+
+def test_block_on_another_stream_and_replayed(k):
+    """The block on a side stream, two blocks on two streams at once, and two captured graphs replayed on new inputs."""
+    M, d, ff = 325, 256, 1024
+    blocks = [block_state(k, M, d, ff, 70 + i) for i in range(2)]
+    want = []
+    for b in blocks:
+        block(k, b)
+        want.append([b[n].clone() for n in ("out", "q", "q2", "h")])
+    torch.cuda.synchronize()
+    side = [torch.cuda.Stream() for _ in blocks]
+    for _ in range(5):
+        for b, s in zip(blocks, side):
+            s.wait_stream(torch.cuda.current_stream())
+            with torch.cuda.stream(s):
+                b["out"].zero_()
+                block(k, b)
+    torch.cuda.synchronize()
+    for b, w in zip(blocks, want):
+        assert all(torch.equal(b[n], t) for n, t in zip(("out", "q", "q2", "h"), w))
+    graphs = []
+    for b in blocks:
+        g = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(g):
+            block(k, b)
+        graphs.append(g)
+    blocks[0]["x"].copy_(blocks[1]["x"])
+    blocks[0]["delta"].copy_(blocks[1]["delta"])
+    for n in ("g", "W1", "c1", "b1", "W2", "c2", "b2"):
+        blocks[0][n].copy_(blocks[1][n])
+    for _ in range(3):
+        for g, s in zip(graphs, side):
+            s.wait_stream(torch.cuda.current_stream())
+            with torch.cuda.stream(s):
+                g.replay()
+        torch.cuda.synchronize()
+        for b in blocks:
+            assert all(torch.equal(b[n], t) for n, t in zip(("out", "q", "q2", "h"), want[1]))
+    del graphs
+
+
+def test_no_rows(k):
+    e = lambda *n, dtype=torch.float32: torch.empty(*n, dtype=dtype, device="cuda")  # noqa: E731
+    k.k_quant_i8(e(0, 64), e(0, 64, dtype=torch.int8), e(0))
+    k.k_rmsnorm_i8(e(0, 64), e(0, 64), e(64), e(0, 64), e(0, 64, dtype=torch.int8), e(0))
+    k.k_gemm_i8(e(0, 64, dtype=torch.int8), torch.ones(8, 64, dtype=torch.int8, device="cuda"), e(0), e(8), None,
+                e(0, 8), 3)
+    torch.cuda.synchronize()
+
+
+# ------------------------------------------------------------------------------------------------ refusals
+def test_wrapper_refusals(k):
+    e = lambda *n, dtype=torch.float32: torch.empty(*n, dtype=dtype, device="cuda")  # noqa: E731
+    i8 = torch.int8
+    x, q, s, g = e(4, 32), e(4, 32, dtype=i8), e(4), e(32)
+    for bad in ((x.double(), q, s), (x.cpu(), q, s), (x, q.cpu(), s), (x, q.float(), s), (x, q[:, :16], s), (x, q, e(5)),
+                (x, q, s.half()), (x, q, e(8)[::2]), (x.t(), q, s), (e(32, 4).t(), q, s), (x[0], q[0], s)):
+        with pytest.raises(ValueError):
+            k.k_quant_i8(*bad)
+    for bad in ((x, None, g, x, q, s), (x, x, g, None, q, s), (x, x, g, x.half(), q, s), (x, x[:2], g, x, q, s),
+                (x, x, e(31), x, q, s), (x, x.double(), g, x, q, s)):
+        with pytest.raises(ValueError):
+            k.k_rmsnorm_i8(*bad)
+    h = x.half()
+    with pytest.raises(RuntimeError, match="delta must be of x's type"):
+        k.k_rmsnorm_i8(h, x, g, h, q, s)
+    for eps in (0.0, -1e-6, math.nan, math.inf):
+        with pytest.raises(RuntimeError, match="eps"):
+            k.k_rmsnorm_i8(x, None, g, None, q, s, eps)
+    with pytest.raises(RuntimeError, match="32768"):
+        k.k_quant_i8(e(1, 32769), e(1, 32769, dtype=i8), e(1))
+    A, W, C = e(4, 32, dtype=i8), e(8, 32, dtype=i8), e(4, 8)
+    c = e(8)
+    for bad in ((A, W[:, :16], s, c, None, C, 3), (A, W, s, c, None, C.t(), 3), (A, W, s, c, None, C, 0),
+                (A, W, s, c, None, C.half(), 2), (A.float(), W, s, c, None, C, 3), (A, W, e(3), c, None, C, 3),
+                (A, W, s, e(4), None, C, 3), (A, W, s, c, e(7), C, 3), (A, W.cpu(), s, c, None, C, 3)):
+        with pytest.raises(ValueError):
+            k.k_gemm_i8(*bad)
+    with pytest.raises(RuntimeError, match="16"):
+        k.k_gemm_i8(e(4, 33, dtype=i8)[:, 1:], W, s, c, None, C, 3)
+    with pytest.raises(RuntimeError, match="multiples of 16"):
+        k.k_gemm_i8(e(4, 40, dtype=i8)[:, :32], W, s, c, None, C, 3)
+    with pytest.raises(RuntimeError, match="epi"):
+        k.k_gemm_i8(A, W, s, c, None, C, 4)
+    with pytest.raises(RuntimeError, match="kernel"):
+        k.k_gemm_i8(A, W, s, c, None, C, 3, 99)
