@@ -227,10 +227,17 @@ CUDANET_API int cudanet_k_quant_i8(int x_type, const void* x, void* q, float* sc
  * int32 sum (any int8 codes, -128 included; 1 <= K <= 131,071, the largest K whose sums fit), with epi as for
  * cudanet_k_gemm: 0: C 16-bit (`dtype`) = v; 1: C 16-bit = gelu(v); 2: C f32 += v; 3: C f32 = v. A and W begin on 16
  * bytes and their row pitches are multiples of 16; C, bias and the scales may begin anywhere and C have any pitch
- * >= N. kernel -1 chooses. Every kernel gives the same bits. */
+ * >= N. kernel -1 chooses; 0 asks for single-CTA 128 x 256 tiles, 1 for CTA-pair 256 x 256 tiles. Every kernel gives the
+ * same bits. M and N up to 2^30. A wait inside the kernel that runs out (a failure of the device) ends it with C
+ * unwritten and is reported by cudanet_k_i8_check. */
 CUDANET_API int cudanet_k_gemm_i8(int dtype, int epi, int kernel, const void* A, const void* W, const float* rowscale,
                                   const float* colscale, const float* bias, void* C, int M, int N, int K, int64_t lda,
                                   int64_t ldw, int64_t ldc, void* stream, char* err, int err_len);
+
+/* Waits for `stream` and reports a failure that a cudanet_k_gemm_i8 call on the current device has recorded since the
+ * last check (one word a device: of any stream). Not to be called while the stream is captured. Returns 0, or -1 with
+ * the reason in err. */
+CUDANET_API int cudanet_k_i8_check(void* stream, char* err, int err_len);
 
 #ifdef __cplusplus
 }

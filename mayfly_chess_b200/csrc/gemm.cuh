@@ -1,7 +1,8 @@
 // The trunk's and the heads' matrix products on the 5th-generation tensor cores (tcgen05, sm_100a).
 //
 //   C[M, N] = A[M, K] * W[N, K]^T  (+ epilogue), A and W 16-bit (f16 or bf16, kind::f16) or e4m3 (the FP8
-//   path, kind::f8f6f4, the accumulator scaled per column in the epilogue), K-major, f32 accumulation.
+//   path, kind::f8f6f4, the accumulator scaled per column in the epilogue), K-major, f32 accumulation; or int8
+//   (kind::i8, s32 accumulation, scaled per row and column; int8.cuh).
 //
 // These are the five products of mayfly/chess/cudanet/cudanet_spec.h:94-101 (qkv, out, ff1, ff2, heads), which
 // the reference runs through cuBLASLt (cudanet/gemm.cpp:209-231) or mma.sync (cudanet/kernels_gemm.cu:99-302).
@@ -47,6 +48,8 @@
 #include <cuda_fp16.h>
 #include <cuda_fp8.h>
 
+#include <type_traits>
+
 #include "ptx.cuh"
 
 // Epilogue groups and staging buffers per group of the f32 residual (added into X by TMA reductions).
@@ -78,34 +81,40 @@ enum Epi : int { kEpiBias = 0, kEpiBiasGelu = 1, kEpiResidual = 2, kEpiF32 = 3, 
 // the FP8 qkv product, slower on the 16-bit products and the residuals' reduce-adds, measured).
 __host__ __device__ constexpr int store_rows(int epi, bool f8) { return epi == kEpiBias && f8 ? 32 : 128; }
 
-// Operand types: 16-bit (kind::f16) or e4m3 (kind::f8f6f4). A stage row is always 128 bytes (the swizzle atom),
-// so an FP8 stage holds 128 elements of K and each MMA instruction 32 (16 for 16-bit); the byte sizes, smem
-// descriptors and the 32-byte step per instruction are the same.
+// Operand types: 16-bit (kind::f16), e4m3 (kind::f8f6f4) or int8 (kind::i8). A stage row is always 128 bytes (the
+// swizzle atom), so a stage of bytes (F8: e4m3 or int8) holds 128 elements of K and each MMA instruction 32 (16 for
+// 16-bit); the byte sizes, smem descriptors and the 32-byte step per instruction are the same.
 template <typename T> struct Operand;
 template <> struct Operand<__half> {
-    static constexpr bool F8 = false;
+    static constexpr bool F8 = false, I8 = false;
     __host__ __device__ static constexpr uint32_t idesc(uint32_t M, uint32_t N) { return idesc_f16(0, M, N); }
 };
 template <> struct Operand<__nv_bfloat16> {
-    static constexpr bool F8 = false;
+    static constexpr bool F8 = false, I8 = false;
     __host__ __device__ static constexpr uint32_t idesc(uint32_t M, uint32_t N) { return idesc_f16(1, M, N); }
 };
 template <> struct Operand<__nv_fp8_e4m3> {
-    static constexpr bool F8 = true;
+    static constexpr bool F8 = true, I8 = false;
     __host__ __device__ static constexpr uint32_t idesc(uint32_t M, uint32_t N) { return idesc_e4m3(M, N); }
+};
+template <> struct Operand<int8_t> {
+    static constexpr bool F8 = true, I8 = true;
+    __host__ __device__ static constexpr uint32_t idesc(uint32_t M, uint32_t N) { return idesc_i8(M, N); }
 };
 
 template <typename TI>
 __device__ __forceinline__ void umma_issue(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc, uint32_t acc)
 {
-    if constexpr (Operand<TI>::F8) umma_f8(d, a, b, idesc, acc);
+    if constexpr (Operand<TI>::I8) umma_i8(d, a, b, idesc, acc);
+    else if constexpr (Operand<TI>::F8) umma_f8(d, a, b, idesc, acc);
     else umma_f16(d, a, b, idesc, acc);
 }
 
 template <typename TI>
 __device__ __forceinline__ void umma_issue_pair(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc, uint32_t acc)
 {
-    if constexpr (Operand<TI>::F8) umma_f8_pair(d, a, b, idesc, acc);
+    if constexpr (Operand<TI>::I8) umma_i8_pair(d, a, b, idesc, acc);
+    else if constexpr (Operand<TI>::F8) umma_f8_pair(d, a, b, idesc, acc);
     else umma_f16_pair(d, a, b, idesc, acc);
 }
 
@@ -116,11 +125,16 @@ struct EpiArgs {
     const float* colscale;   // nullptr: no scaling (16-bit operands)
     float out_scale_inv;     // kEpiGeluE4m3 only
     int rev;                 // 1: the M blocks in descending order (the output is the same)
+    // int8 products only
+    const float* rowscale;   // [M]
+    void* direct;            // C, where its start or pitch do not suit TMA stores; else nullptr
+    long long ldc;           // C's pitch (elements), for `direct`
+    int vec;                 // colscale and bias begin on 16 bytes
 };
 
 // PAIR: the CTA-pair kernel, where a CTA loads BN/2 rows of W per stage and a pair covers 256 rows of M.
-// F8: e4m3 operands (128 elements of K per stage instead of 64; the same bytes).
-template <int BN, int EPI, bool PAIR = false, bool F8 = false> struct GemmCfg {
+// F8: byte operands (128 elements of K per stage instead of 64; the same bytes). I8: they are int8.
+template <int BN, int EPI, bool PAIR = false, bool F8 = false, bool I8 = false> struct GemmCfg {
     static constexpr int BM = 128;                      // rows of A and of the output per CTA
     static constexpr int BK = F8 ? 128 : 64;            // elements of K per stage: one 128-byte swizzle row
     static constexpr int KSTEPS = 4;                    // MMA instructions per stage (K = 16 or 32 each, 32 bytes)
@@ -128,7 +142,7 @@ template <int BN, int EPI, bool PAIR = false, bool F8 = false> struct GemmCfg {
     // the residuals are added into X by a TMA reduction at L2 (f32 adds for the f32 stream, bf16 adds of the
     // bf16-rounded v for the bf16 stream), so X is neither read into the SM nor staged
     static constexpr bool REDUCE = EPI == kEpiResidual || EPI == kEpiResidual16;
-    static constexpr bool IS_F8 = F8;
+    static constexpr bool IS_F8 = F8, IS_I8 = I8;
     static constexpr bool HEAVY = EPI == kEpiBiasGelu || EPI == kEpiGeluE4m3;   // GELU's erf per element
     static constexpr int OUT_BYTES = (EPI == kEpiResidual || EPI == kEpiF32) ? 4 : (EPI == kEpiGeluE4m3 ? 1 : 2);
     // one staging chunk: 128 rows x ROW_BYTES (64-byte rows for the GELU epilogues, whose four groups each take
@@ -328,6 +342,46 @@ __device__ __forceinline__ void scale_bias32(float (&v)[NV], int off, const floa
     }
 }
 
+// The int8 products' value of one accumulator before GELU or a residual's addition, a rounding a step and the same in
+// every kernel, so that they agree to the bit.
+__device__ __forceinline__ float i8_value(int acc, float rowscale, float colscale, float bias)
+{
+    return fmaf(__fmul_rn(__int2float_rn(acc), rowscale), colscale, bias);
+}
+
+// v[i] = i8_value of accumulator r[i] of column col0 + i, i < 32. bias nullptr: 0 (a result of -0 becomes +0 with it).
+__device__ __forceinline__ void scale_i8_32(float (&v)[32], const uint32_t (&r)[32], float rowscale, const EpiArgs& ep,
+                                            int col0, int N)
+{
+    if (col0 + 32 <= N && ep.vec) {
+        const float4* s4 = reinterpret_cast<const float4*>(ep.colscale + col0);
+        const float4* b4 = reinterpret_cast<const float4*>(ep.bias + col0);
+        const uint64_t rs2 = pk2(rowscale, rowscale);
+        const bool has_bias = ep.bias != nullptr;
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+            const float4 sc = __ldg(s4 + i);
+            const float4 b = has_bias ? __ldg(b4 + i) : make_float4(0.f, 0.f, 0.f, 0.f);
+            const float2 lo = upk2(fma2(mul2(pk2(__int2float_rn((int)r[4 * i]), __int2float_rn((int)r[4 * i + 1])), rs2),
+                                        pk2(sc.x, sc.y), pk2(b.x, b.y)));
+            const float2 hi =
+                upk2(fma2(mul2(pk2(__int2float_rn((int)r[4 * i + 2]), __int2float_rn((int)r[4 * i + 3])), rs2),
+                          pk2(sc.z, sc.w), pk2(b.z, b.w)));
+            v[4 * i + 0] = lo.x;
+            v[4 * i + 1] = lo.y;
+            v[4 * i + 2] = hi.x;
+            v[4 * i + 3] = hi.y;
+        }
+    } else {
+#pragma unroll
+        for (int i = 0; i < 32; ++i) {
+            const bool in = col0 + i < N;
+            v[i] = i8_value((int)r[i], rowscale, in ? __ldg(ep.colscale + col0 + i) : 0.f,
+                            in && ep.bias ? __ldg(ep.bias + col0 + i) : 0.f);
+        }
+    }
+}
+
 // four floats to four e4m3 bytes (round to nearest even, saturating to +-448), first value in the lowest byte
 __device__ __forceinline__ uint32_t pack_e4m3x4(float a, float b, float c, float d)
 {
@@ -401,7 +455,7 @@ __device__ __forceinline__ void epilogue_loop(const SmemLayout<C>& L, const CUte
         if (it < my_tiles && gtid < BN / 32) {
             const int c = origin_col(it) + 32 * gtid;
             if (c < N) {
-                asm volatile("prefetch.global.L1 [%0];" ::"l"(bias + c));
+                if (!C::IS_I8 || bias) asm volatile("prefetch.global.L1 [%0];" ::"l"(bias + c));
                 if constexpr (C::IS_F8) asm volatile("prefetch.global.L1 [%0];" ::"l"(colscale + c));
             }
         }
@@ -413,6 +467,9 @@ __device__ __forceinline__ void epilogue_loop(const SmemLayout<C>& L, const CUte
     int g = 0;        // this group's chunks done
     for (int it = 0; it < my_tiles; ++it) {
         const int row0 = origin_row(it), colb = origin_col(it);
+        float rowscale = 0.f;   // read before the wait for the accumulator, which hides it
+        if constexpr (C::IS_I8)
+            if (row0 + row < M) rowscale = __ldg(ep.rowscale + row0 + row);
         prefetch_bias(it + 1);
         if (leader) L.epi_ok[grp] = mbar_wait(&L.tfull[acc], acc_phase, err, kErrTmemFull) ? 1u : 0u;
         named_barrier(bar_id, 128);
@@ -442,15 +499,18 @@ __device__ __forceinline__ void epilogue_loop(const SmemLayout<C>& L, const CUte
                     if (lane == 0) release(acc);
                 }
                 constexpr int off = 0;
+                if constexpr (!C::IS_I8) {
 #pragma unroll
-                for (int i = 0; i < 32; ++i) v[off + i] = __uint_as_float(r[i]);
-                if constexpr (C::IS_F8) scale_bias32(v, off, colscale, bias, col0 + 32 * p, N);
+                    for (int i = 0; i < 32; ++i) v[off + i] = __uint_as_float(r[i]);
+                }
+                if constexpr (C::IS_I8) scale_i8_32(v, r, rowscale, ep, col0 + 32 * p, N);
+                else if constexpr (C::IS_F8) scale_bias32(v, off, colscale, bias, col0 + 32 * p, N);
                 else add_bias32(v, off, bias, col0 + 32 * p, N);
                 if constexpr (EPI == kEpiBiasGelu) {
                     const GeluK K(1.0f);
 #pragma unroll
                     for (int i = 0; i < 16; ++i) {
-                        const float2 g = gelu_pair(pk2(v[2 * i], v[2 * i + 1]), K);
+                        const float2 g = gelu_pair<false, C::IS_I8>(pk2(v[2 * i], v[2 * i + 1]), K);
                         q[16 * p + i] = pack2<T>(g.x, g.y);
                     }
                 } else if constexpr (EPI == kEpiGeluE4m3) {
@@ -494,6 +554,29 @@ __device__ __forceinline__ void epilogue_loop(const SmemLayout<C>& L, const CUte
                     *reinterpret_cast<uint4*>(buf + swz<RB>(row, j)) =
                         make_uint4(q[4 * j], q[4 * j + 1], q[4 * j + 2], q[4 * j + 3]);
             }
+            if constexpr (C::IS_I8) {
+                if (ep.direct) {
+                    // C does not suit TMA: each warp writes the 32 rows that it staged, a row's columns by its lanes
+                    using TO = std::conditional_t<C::OUT_BYTES == 4, float, T>;
+                    TO* c = static_cast<TO*>(ep.direct);
+                    __syncwarp();
+                    for (int i = 0; i < 32 && row0 + quarter * 32 + i < M; ++i) {
+                        const int rr = quarter * 32 + i;
+                        TO* crow = c + (size_t)(row0 + rr) * ep.ldc;
+#pragma unroll
+                        for (int j = lane; j < C::CHUNK_COLS; j += 32) {
+                            constexpr int PER = 16 / C::OUT_BYTES;   // elements of a 16-byte unit
+                            const TO e = reinterpret_cast<const TO*>(buf + swz<RB>(rr, j / PER))[j % PER];
+                            if (col0 + j < N) {
+                                if constexpr (EPI == kEpiResidual) crow[col0 + j] += e;
+                                else crow[col0 + j] = e;
+                            }
+                        }
+                    }
+                    __syncwarp();   // read, before the next chunk overwrites it
+                    continue;
+                }
+            }
             if (C::BATCH && ci < CPG - 1) continue;   // batched: the fence and the stores after the last chunk
             fence_proxy_async_smem();
             constexpr int NST = C::BATCH ? CPG : 1;   // chunks this fence covers: ci - NST + 1 .. ci
@@ -532,11 +615,11 @@ __device__ __forceinline__ void epilogue_loop(const SmemLayout<C>& L, const CUte
 // ------------------------------------------------------------------------------------------------ one CTA
 // TI: the operands' type (f16, bf16 or e4m3); T: the 16-bit output type of kEpiBias / kEpiBiasGelu.
 template <typename TI, typename T, int BN, int EPI>
-__global__ void __launch_bounds__(GemmCfg<BN, EPI, false, Operand<TI>::F8>::THREADS, 1)
+__global__ void __launch_bounds__(GemmCfg<BN, EPI, false, Operand<TI>::F8, Operand<TI>::I8>::THREADS, 1)
 gemm_tc_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant__ CUtensorMap tmB,
                const __grid_constant__ CUtensorMap tmC, int M, int N, int K, const EpiArgs ep, uint32_t* err)
 {
-    using C = GemmCfg<BN, EPI, false, Operand<TI>::F8>;
+    using C = GemmCfg<BN, EPI, false, Operand<TI>::F8, Operand<TI>::I8>;
     extern __shared__ uint8_t smem_raw[];
     const SmemLayout<C> L(smem_raw);
 
@@ -544,7 +627,7 @@ gemm_tc_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant__ 
     const int m_tiles = (M + C::BM - 1) / C::BM;
     const int n_tiles = (N + BN - 1) / BN;
     const int num_tiles = m_tiles * n_tiles;
-    const int k_iters = K / C::BK;
+    const int k_iters = C::IS_I8 ? (K + C::BK - 1) / C::BK : K / C::BK;   // int8: TMA fills K's tail with zeros
 
     if (threadIdx.x == 0) {
         for (int s = 0; s < C::STAGES; ++s) {
@@ -581,7 +664,8 @@ gemm_tc_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant__ 
             bool ok = true;
             // the weight tiles of this CTA's first stages depend on no earlier kernel: they load while that
             // kernel finishes; A (an earlier kernel's output) only after griddep_wait
-            const int pre = (int)blockIdx.x < num_tiles ? (k_iters < C::STAGES ? k_iters : C::STAGES) : 0;
+            // (int8 products are queued by themselves: the kernel before one may write its weights)
+            const int pre = !C::IS_I8 && (int)blockIdx.x < num_tiles ? (k_iters < C::STAGES ? k_iters : C::STAGES) : 0;
             for (int kb = 0; kb < pre; ++kb) {
                 mbar_arrive_expect_tx(&L.full[kb], C::STAGE_BYTES);
                 tma_load_2d(L.sB + kb * C::B_BYTES, &tmB, &L.full[kb], kb * C::BK, ((int)blockIdx.x % n_tiles) * BN);
@@ -677,12 +761,12 @@ gemm_tc_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant__ 
 // CTAs' loads complete there), the accumulator's `tempty` barriers (both CTAs' epilogue warps arrive there) and
 // issues every MMA; each CTA's `empty` and `tfull` barriers are signalled by the leader's commits.
 template <typename TI, typename T, int EPI>
-__global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(GemmCfg<256, EPI, true, Operand<TI>::F8>::THREADS, 1)
+__global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(GemmCfg<256, EPI, true, Operand<TI>::F8, Operand<TI>::I8>::THREADS, 1)
 gemm_tc_pair_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant__ CUtensorMap tmB,
                     const __grid_constant__ CUtensorMap tmC, int M, int N, int K, const EpiArgs ep, uint32_t* err)
 {
     constexpr int BN = 256;
-    using C = GemmCfg<BN, EPI, true, Operand<TI>::F8>;
+    using C = GemmCfg<BN, EPI, true, Operand<TI>::F8, Operand<TI>::I8>;
     extern __shared__ uint8_t smem_raw[];
     const SmemLayout<C> L(smem_raw);
 
@@ -693,7 +777,7 @@ gemm_tc_pair_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_consta
     const int m_tiles = (M + 2 * C::BM - 1) / (2 * C::BM);
     const int n_tiles = (N + BN - 1) / BN;
     const int num_tiles = m_tiles * n_tiles;
-    const int k_iters = K / C::BK;
+    const int k_iters = C::IS_I8 ? (K + C::BK - 1) / C::BK : K / C::BK;   // int8: TMA fills K's tail with zeros
 
     if (threadIdx.x == 0) {
         for (int s = 0; s < C::STAGES; ++s) {
@@ -728,7 +812,7 @@ gemm_tc_pair_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_consta
             uint32_t issued = 0, issued_par = 0;
             bool ok = true;
             // this CTA's half of the first stages' weight tiles loads before griddep_wait (as in gemm_tc_kernel)
-            const int pre = pair < num_tiles ? (k_iters < C::STAGES ? k_iters : C::STAGES) : 0;
+            const int pre = !C::IS_I8 && pair < num_tiles ? (k_iters < C::STAGES ? k_iters : C::STAGES) : 0;
             for (int kb = 0; kb < pre; ++kb) {
                 if (lead) mbar_arrive_expect_tx(&L.full[kb], 2 * C::STAGE_BYTES);
                 tma_load_2d_pair(L.sB + kb * C::B_BYTES, &tmB, mapa_shared(smem_u32(&L.full[kb]), 0), kb * C::BK,

@@ -91,12 +91,6 @@ __global__ void __launch_bounds__(256) rows_i8_kernel(const XT* __restrict__ x, 
     if (threadIdx.x == 0) scale[row] = rs.scale;
 }
 
-// The epilogue's value before GELU, one rounding a step in every kernel, so that they agree to the bit.
-__device__ __forceinline__ float i8_value(int acc, float rowscale, float colscale, float bias)
-{
-    return fmaf(__fmul_rn(__int2float_rn(acc), rowscale), colscale, bias);
-}
-
 // One thread an output, 16 x 16 outputs a block, K by 64 codes through shared memory.
 template <typename TO, int EPI>
 __global__ void __launch_bounds__(256) gemm_i8_simple_kernel(const int8_t* __restrict__ A, const int8_t* __restrict__ W,

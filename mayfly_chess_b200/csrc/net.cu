@@ -127,7 +127,7 @@ static CUtensorMap operand_map(const void* base, MapType type, uint64_t K, uint6
 // boxes of one epilogue store (GemmCfg::ROW_BYTES wide: 64-byte rows for the GELU epilogues, the bf16 residual
 // and the bias epilogue of an FP8 product, `f8`; store_rows(epi, f8) rows high). The residuals' maps take TMA
 // reduce-adds into X.
-static CUtensorMap output_map(void* base, int epi, MapType t16, int M, int N, int ldc, bool f8 = false)
+static CUtensorMap output_map(void* base, int epi, MapType t16, int M, int N, long long ldc, bool f8 = false)
 {
     const uint32_t rows = static_cast<uint32_t>(store_rows(epi, f8));
     if (epi == kEpiResidual || epi == kEpiF32) return make_map(base, MapType::F32, N, M, ldc, 32, rows);
@@ -171,7 +171,7 @@ template <typename TI, typename T, int BN, int EPI>
 static void launch_gemm_bn(const CUtensorMap& ma, const CUtensorMap& mb, const CUtensorMap& mc, int M, int N, int K,
                            const EpiArgs& ep, uint32_t* err, int num_sms, cudaStream_t s)
 {
-    using C = GemmCfg<BN, EPI, false, Operand<TI>::F8>;
+    using C = GemmCfg<BN, EPI, false, Operand<TI>::F8, Operand<TI>::I8>;
     // the shared-memory opt-in, once per instantiation and device (the first launch of a batch size is eager,
     // never inside a graph capture)
     static bool attr[64] = {};
@@ -194,7 +194,7 @@ template <typename TI, typename T, int EPI>
 static void launch_gemm_pair(const CUtensorMap& ma, const CUtensorMap& mb, const CUtensorMap& mc, int M, int N,
                              int K, const EpiArgs& ep, uint32_t* err, cudaStream_t s)
 {
-    using C = GemmCfg<256, EPI, true, Operand<TI>::F8>;
+    using C = GemmCfg<256, EPI, true, Operand<TI>::F8, Operand<TI>::I8>;
     static int max_pairs[64] = {};
     int dev = 0;
     RT(cudaGetDevice(&dev));
@@ -1653,7 +1653,26 @@ static void attention_once(const void* qkv, void* att, int B, int d, int heads, 
 // The element types of the int8 entry points: the codes of the 16-bit kernels, and 2 = f32.
 enum I8Type : int { kI8F16 = 0, kI8BF16 = 1, kI8F32 = 2 };
 constexpr int kI8MaxRow = 32768;    // the longest row of the norm and the quantiser
+constexpr int kI8MaxRows = 1 << 30; // rows of A and of W: tile counts and rounded-up sizes stay within int
 constexpr int kI8MaxK = 131071;     // 131,071 products of -128 * -128 are the most that an int32 sum holds
+
+// The word that the int8 products' bounded waits report in, one on every GPU that loads the library: 0, or the first
+// failure since cudanet_k_i8_check last read it.
+static __device__ uint32_t g_i8_error;
+
+static uint32_t* i8_error_word(int dev)
+{
+    static std::mutex mu;
+    static uint32_t* addr[64] = {};
+    if (dev < 0 || dev >= 64) throw std::runtime_error("cudanet_b200: device index out of range");
+    std::lock_guard<std::mutex> lock(mu);
+    if (!addr[dev]) {
+        void* p = nullptr;
+        RT(cudaGetSymbolAddress(&p, g_i8_error));
+        addr[dev] = static_cast<uint32_t*>(p);
+    }
+    return addr[dev];
+}
 
 static long long i8_bytes(int type) { return type == kI8F32 ? 4 : 2; }
 
@@ -1683,14 +1702,49 @@ static void launch_rows_i8(int x_type, int delta_type, const void* x, const void
     else go(float(), __nv_bfloat16());
 }
 
-template <typename TO, int EPI>
-static void launch_gemm_i8_t(const void* A, const void* W, const float* rowscale, const float* colscale,
-                             const float* bias, void* C, int M, int N, int K, long long lda, long long ldw,
-                             long long ldc, cudaStream_t s)
+// What an int8 product is called with.
+struct GemmI8 {
+    const void *A, *W;
+    const float *rowscale, *colscale, *bias;
+    void* C;
+    int M, N, K;
+    long long lda, ldw, ldc;
+};
+
+// The kernels of an int8 product: the choice of `kernel` -1, else what the caller asks for.
+enum I8Kernel : int { kI8Single = 0, kI8Pair = 1 };
+
+static int pick_i8_kernel(const GemmI8& p, int num_sms)
 {
-    launch_k(gemm_i8_simple_kernel<TO, EPI>, dim3((N + 15) / 16, (M + 15) / 16), dim3(256), 0, s,
-             static_cast<const int8_t*>(A), static_cast<const int8_t*>(W), rowscale, colscale, bias,
-             static_cast<TO*>(C), M, N, K, lda, ldw, ldc);
+    const long long tiles = ((p.M + 255LL) / 256) * ((p.N + 255) / 256);
+    return tiles >= num_sms / 2 ? kI8Pair : kI8Single;
+}
+
+template <typename TO, int EPI>
+static void launch_gemm_i8_t(const GemmI8& p, int kernel, cudaStream_t s)
+{
+    using T = std::conditional_t<std::is_same<TO, float>::value, __nv_bfloat16, TO>;   // not used by f32 outputs
+    int dev = 0, sms = 0;
+    RT(cudaGetDevice(&dev));
+    RT(cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, dev));
+    if (kernel < 0) kernel = pick_i8_kernel(p, sms);
+    const auto pitch = [](long long ld, int width, int rows) { return rows > 1 ? ld : (width + 15LL) / 16 * 16; };
+    const CUtensorMap ma = make_map(p.A, MapType::U8, p.K, p.M, pitch(p.lda, p.K, p.M), 128, 128);
+    const CUtensorMap mb = make_map(p.W, MapType::U8, p.K, p.N, pitch(p.ldw, p.K, p.N), 128,
+                                    w_box_rows(kernel == kI8Pair ? kPairTile : 256));
+    // a TMA store writes whole 16-byte units, the last of a row past its end too: rows must be made of such units
+    const bool tma_out = reinterpret_cast<uintptr_t>(p.C) % 16 == 0 && p.N * sizeof(TO) % 16 == 0 &&
+                         (p.M == 1 || p.ldc * sizeof(TO) % 16 == 0);
+    // with direct stores the kernel never uses the output's map: any valid one
+    const CUtensorMap mc = tma_out ? output_map(p.C, EPI, type16(std::is_same<T, __nv_bfloat16>::value), p.M, p.N,
+                                                pitch(p.ldc, p.N, p.M), true)
+                                   : ma;
+    const auto low = reinterpret_cast<uintptr_t>(p.colscale) | reinterpret_cast<uintptr_t>(p.bias);
+    const EpiArgs ep{p.bias, p.colscale, 1.f, 0, p.rowscale, tma_out ? nullptr : p.C, p.ldc, low % 16 == 0};
+    if (kernel == kI8Pair)
+        launch_gemm_pair<int8_t, T, EPI>(ma, mb, mc, p.M, p.N, p.K, ep, i8_error_word(dev), s);
+    else
+        launch_gemm_bn<int8_t, T, 256, EPI>(ma, mb, mc, p.M, p.N, p.K, ep, i8_error_word(dev), sms, s);
 }
 
 // A null pointer, or one whose address is no multiple of `align`, named in the reason.
@@ -2275,9 +2329,9 @@ CUDANET_API int cudanet_k_gemm_i8(int dtype, int epi, int kernel, const void* A,
         const char* who = "cudanet_k_gemm_i8";
         if (dtype != 0 && dtype != 1) throw std::runtime_error(std::string(who) + ": dtype must be 0 (f16) or 1 (bf16)");
         if (epi < 0 || epi > 3) throw std::runtime_error(std::string(who) + ": epi must be 0..3");
-        if (kernel != -1) throw std::runtime_error(std::string(who) + ": kernel must be -1");
-        if (M < 0 || N < 1 || K < 1 || K > mf::kI8MaxK)
-            throw std::runtime_error(std::string(who) + ": bad sizes (M >= 0, N >= 1, 1 <= K <= 131071)");
+        if (kernel < -1 || kernel > 1) throw std::runtime_error(std::string(who) + ": kernel must be -1, 0 or 1");
+        if (M < 0 || N < 1 || K < 1 || K > mf::kI8MaxK || M > mf::kI8MaxRows || N > mf::kI8MaxRows)
+            throw std::runtime_error(std::string(who) + ": bad sizes (0 <= M, 1 <= N, both <= 2^30, 1 <= K <= 131071)");
         if (M == 0) return 0;
         mf::need_ptr(who, "A", A, 16);
         mf::need_ptr(who, "W", W, 16);
@@ -2292,8 +2346,8 @@ CUDANET_API int cudanet_k_gemm_i8(int dtype, int epi, int kernel, const void* A,
             throw std::runtime_error(std::string(who) + ": the row pitches of A and W must be multiples of 16 bytes");
         const cudaStream_t s = static_cast<cudaStream_t>(stream);
         auto go = [&](auto to, auto e) {
-            mf::launch_gemm_i8_t<decltype(to), decltype(e)::value>(A, W, rowscale, colscale, bias, C, M, N, K, lda,
-                                                                   ldw, ldc, s);
+            mf::launch_gemm_i8_t<decltype(to), decltype(e)::value>(
+                {A, W, rowscale, colscale, bias, C, M, N, K, lda, ldw, ldc}, kernel, s);
         };
         using E0 = std::integral_constant<int, mf::kEpiBias>;
         using E1 = std::integral_constant<int, mf::kEpiBiasGelu>;
@@ -2301,6 +2355,25 @@ CUDANET_API int cudanet_k_gemm_i8(int dtype, int epi, int kernel, const void* A,
         else if (epi == mf::kEpiF32) go(float(), std::integral_constant<int, mf::kEpiF32>());
         else if (dtype == 1) epi == 0 ? go(__nv_bfloat16(), E0()) : go(__nv_bfloat16(), E1());
         else epi == 0 ? go(__half(), E0()) : go(__half(), E1());
+        return 0;
+    });
+}
+
+CUDANET_API int cudanet_k_i8_check(void* stream, char* err, int err_len)
+{
+    return mf::guarded(err, err_len, "cudanet_k_i8_check: unknown exception", [&] {
+        int dev = 0;
+        mf::RT(cudaGetDevice(&dev));
+        uint32_t* word = mf::i8_error_word(dev);
+        const cudaStream_t s = static_cast<cudaStream_t>(stream);
+        uint32_t e = 0;
+        mf::RT(cudaMemcpyAsync(&e, word, sizeof e, cudaMemcpyDeviceToHost, s));
+        mf::RT(cudaStreamSynchronize(s));
+        if (e) {
+            mf::RT(cudaMemsetAsync(word, 0, sizeof e, s));
+            mf::RT(cudaStreamSynchronize(s));
+            throw std::runtime_error(std::string("cudanet_k_gemm_i8: device error: ") + mf::err_site_name(e >> 8));
+        }
         return 0;
     });
 }

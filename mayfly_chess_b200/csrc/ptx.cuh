@@ -224,6 +224,18 @@ __device__ __forceinline__ void umma_f8(uint32_t d_tmem, uint64_t a_desc, uint64
         : "memory");
 }
 
+// The same for signed 8-bit integers (kind::i8), s32 accumulator: exact.
+__device__ __forceinline__ void umma_i8(uint32_t d_tmem, uint64_t a_desc, uint64_t b_desc, uint32_t idesc,
+                                        uint32_t accumulate)
+{
+    asm volatile(
+        "{\n\t.reg .pred p;\n\t"
+        "setp.ne.b32 p, %4, 0;\n\t"
+        "tcgen05.mma.cta_group::1.kind::i8 [%0], %1, %2, %3, p;\n\t}"
+        ::"r"(d_tmem), "l"(a_desc), "l"(b_desc), "r"(idesc), "r"(accumulate)
+        : "memory");
+}
+
 // Arrive once on the barrier when every tcgen05.mma this thread issued before has completed.
 __device__ __forceinline__ void umma_commit(uint64_t* bar)
 {
@@ -316,6 +328,18 @@ __device__ __forceinline__ void umma_f8_pair(uint32_t d_tmem, uint64_t a_desc, u
         : "memory");
 }
 
+// The same for signed 8-bit integers (kind::i8, s32 accumulator), issued by the leader CTA only.
+__device__ __forceinline__ void umma_i8_pair(uint32_t d_tmem, uint64_t a_desc, uint64_t b_desc, uint32_t idesc,
+                                             uint32_t accumulate)
+{
+    asm volatile(
+        "{\n\t.reg .pred p;\n\t"
+        "setp.ne.b32 p, %4, 0;\n\t"
+        "tcgen05.mma.cta_group::2.kind::i8 [%0], %1, %2, %3, p;\n\t}"
+        ::"r"(d_tmem), "l"(a_desc), "l"(b_desc), "r"(idesc), "r"(accumulate)
+        : "memory");
+}
+
 // Arrive once on a barrier of either CTA of the pair when the pair MMAs this thread issued have completed.
 __device__ __forceinline__ void umma_commit_pair(uint32_t bar_cluster_addr)
 {
@@ -395,6 +419,12 @@ __host__ __device__ constexpr uint32_t idesc_f16(uint32_t ab_format, uint32_t M,
 __host__ __device__ constexpr uint32_t idesc_e4m3(uint32_t M, uint32_t N)
 {
     return (1u << 4) | (0u << 7) | (0u << 10) | ((N >> 3) << 17) | ((M >> 4) << 24);
+}
+
+// Instruction descriptor of kind::i8, A and B signed (format 1), D s32 (format 2), no saturation, K-major.
+__host__ __device__ constexpr uint32_t idesc_i8(uint32_t M, uint32_t N)
+{
+    return (2u << 4) | (1u << 7) | (1u << 10) | ((N >> 3) << 17) | ((M >> 4) << 24);
 }
 
 }  // namespace mf

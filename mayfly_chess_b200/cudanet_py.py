@@ -119,6 +119,8 @@ def load(dll=None):
         lib.cudanet_k_gemm_i8.argtypes = [i32, i32, i32, vp, vp, vp, vp, vp, vp, i32, i32, i32, i64, i64, i64, vp, cp,
                                           i32]
         lib.cudanet_k_gemm_i8.restype = i32
+        lib.cudanet_k_i8_check.argtypes = [vp, cp, i32]
+        lib.cudanet_k_i8_check.restype = i32
         _libs[path] = lib
         return lib
 
@@ -719,3 +721,13 @@ def k_gemm_i8(A, W, rowscale, colscale, bias, C, epi, kernel=-1, dll=None):
              _i8_vec(rowscale, "rowscale", M, dev), _i8_vec(colscale, "colscale", N, dev),
              None if bias is None else _i8_vec(bias, "bias", N, dev), C.data_ptr(), M, N, K, lda, ldw, ldc)
     return C
+
+
+def k_i8_check(stream=None, dll=None):
+    """Wait for `stream` (a torch.cuda.Stream, default the current one) and raise if a bounded wait of a k_gemm_i8 call
+    on the current device has failed since the last check."""
+    import torch
+    s = stream if stream is not None else torch.cuda.current_stream()
+    err = ctypes.create_string_buffer(ERR_LEN)
+    if load(dll).cudanet_k_i8_check(ctypes.c_void_p(s.cuda_stream), err, ERR_LEN) != 0:
+        raise RuntimeError(f"cudanet_k_i8_check: {_msg(err)}")

@@ -29,7 +29,7 @@ GEMM = ("dtype", "epi", "kernel", "A", "W", "rowscale", "colscale", "bias", "C",
 @pytest.mark.parametrize("reason,change", [
     ("dtype", {"dtype": 2}), ("dtype", {"dtype": -1}), ("epi", {"epi": 4}), ("epi", {"epi": -1}),
     ("kernel", {"kernel": 77}), ("bad sizes", {"M": -1}), ("bad sizes", {"N": 0}), ("bad sizes", {"K": 0}),
-    ("bad sizes", {"K": 131072}), ("A is a null", {"A": None}), ("W is a null", {"W": None}),
+    ("bad sizes", {"K": 131072}), ("bad sizes", {"M": 2 ** 31 - 1}), ("bad sizes", {"N": 2 ** 30 + 1}), ("A is a null", {"A": None}), ("W is a null", {"W": None}),
     ("rowscale is a null", {"rowscale": None}), ("colscale is a null", {"colscale": None}), ("C is a null", {"C": None}),
     ("A is not aligned to 16", {"A": P + 8}), ("W is not aligned to 16", {"W": P + 1}),
     ("rowscale is not aligned to 4", {"rowscale": P + 2}), ("bias is not aligned to 4", {"bias": P + 1}),

@@ -219,6 +219,7 @@ def check_product(C, C0, A, W, rs, cs, bias, epi):
     assert math.isfinite(excess) and excess <= 0, excess
 
 
+KERNELS = (-1, 0, 1)      # the choice of the library and each of its kernels: all give the same bits
 SIZES = [(1, 1, 1), (1, 8324, 1024), (2, 7, 15), (3, 64, 16), (5, 129, 130), (16, 1000, 2048), (17, 100, 31), (33, 257, 4100),
          (65, 2048, 1024), (64, 128, 128), (129, 72, 1000), (128, 256, 64), (300, 1001, 200), (777, 512, 257),
          (1040, 1024, 1024), (4160, 776, 384)]
@@ -237,11 +238,15 @@ def test_gemm(k, M, N, K, epi, out):
         if epi == 2:
             C.copy_(torch.randn(M, N, device="cuda", generator=gen(N)))
         C0 = C.clone()
-        assert k.k_gemm_i8(A, W, rs, cs, bias, C, epi) is C
-        check_product(C, C0, A, W, rs, cs, bias, epi)
-        assert untouched(C, full, 7, off)
-        first = C.clone() if first is None else first
-        assert torch.equal(C, first)
+        for kernel in KERNELS:
+            C.copy_(C0)
+            assert k.k_gemm_i8(A, W, rs, cs, bias, C, epi, kernel) is C
+            if first is None:
+                check_product(C, C0, A, W, rs, cs, bias, epi)
+                first = C.clone()
+            assert torch.equal(C, first), f"kernel {kernel}, pitch {pitch}"
+            assert untouched(C, full, 7, off)
+    k.k_i8_check()
 
 
 @pytest.mark.parametrize("M", [1, 20, 300])
@@ -254,20 +259,22 @@ def test_gemm_largest_sums(k, M):
     W[1].fill_(127)
     C = torch.empty(M, 40, device="cuda")
     one = torch.ones(M, device="cuda"), torch.ones(40, device="cuda")
-    k.k_gemm_i8(A, W, *one, None, C, 3)
     want = torch.full((M, 40), float(128 * 128 * K), device="cuda")
     want[:, 1] = -128.0 * 127 * K
-    assert torch.equal(C, want)
+    for kernel in KERNELS:
+        k.k_gemm_i8(A, W, *one, None, C.zero_(), 3, kernel)
+        assert torch.equal(C, want), kernel
 
 
 def test_gemm_nan_scale_marks_its_row(k):
     A, W, rs, cs, bias = operands(70, 96, 64, 3)
     rs[3] = math.nan
     for out, epi in (("bf16", 0), ("f16", 1), ("f32", 2), ("f32", 3)):
-        C = torch.zeros(70, 96, dtype=DT[out], device="cuda")
-        k.k_gemm_i8(A, W, rs, cs, bias, C, epi)
-        bad = torch.isnan(C)
-        assert bad[3].all() and not bad[[i for i in range(70) if i != 3]].any()
+        for kernel in KERNELS:
+            C = torch.zeros(70, 96, dtype=DT[out], device="cuda")
+            k.k_gemm_i8(A, W, rs, cs, bias, C, epi, kernel)
+            bad = torch.isnan(C)
+            assert bad[3].all() and not bad[[i for i in range(70) if i != 3]].any()
 
 
 def test_gemm_offset_vectors(k):
@@ -275,9 +282,10 @@ def test_gemm_offset_vectors(k):
     A, W, rs, cs, bias = operands(400, 520, 256, 9)
     want = torch.empty(390, 511, dtype=torch.bfloat16, device="cuda")
     k.k_gemm_i8(A[10:], W[9:], rs[10:].clone(), cs[9:].clone(), bias[9:].clone(), want, 0)
-    got = torch.empty_like(want)
-    k.k_gemm_i8(A[10:], W[9:], rs[10:], cs[9:], bias[9:], got, 0)
-    assert torch.equal(got, want)
+    for kernel in KERNELS:
+        got = torch.empty_like(want)
+        k.k_gemm_i8(A[10:], W[9:], rs[10:], cs[9:], bias[9:], got, 0, kernel)
+        assert torch.equal(got, want), kernel
     check_product(got, None, A[10:], W[9:], rs[10:], cs[9:], bias[9:], 0)
 
 
