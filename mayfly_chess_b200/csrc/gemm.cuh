@@ -127,14 +127,12 @@ struct EpiArgs {
     int rev;                 // 1: the M blocks in descending order (the output is the same)
     // int8 products only
     const float* rowscale;   // [M]
-    void* direct;            // C, where its start or pitch do not suit TMA stores; else nullptr
-    long long ldc;           // C's pitch (elements), for `direct`
-    int vec;                 // colscale and bias begin on 16 bytes
 };
 
 // PAIR: the CTA-pair kernel, where a CTA loads BN/2 rows of W per stage and a pair covers 256 rows of M.
 // F8: byte operands (128 elements of K per stage instead of 64; the same bytes). I8: they are int8.
-template <int BN, int EPI, bool PAIR = false, bool F8 = false, bool I8 = false> struct GemmCfg {
+template <int BN_, int EPI, bool PAIR = false, bool F8 = false, bool I8 = false> struct GemmCfg {
+    static constexpr int BN = BN_;
     static constexpr int BM = 128;                      // rows of A and of the output per CTA
     static constexpr int BK = F8 ? 128 : 64;            // elements of K per stage: one 128-byte swizzle row
     static constexpr int KSTEPS = 4;                    // MMA instructions per stage (K = 16 or 32 each, 32 bytes)
@@ -151,7 +149,7 @@ template <int BN, int EPI, bool PAIR = false, bool F8 = false, bool I8 = false> 
     // product, no faster on the 16-bit one; 128-byte rows otherwise)
     static constexpr bool F8_BIAS = EPI == kEpiBias && F8;
     static constexpr bool NARROW = (F8_BIAS && MF_F8_BIAS_NARROW) || EPI == kEpiResidual16;
-    static constexpr int ROW_BYTES = (HEAVY || NARROW) ? 64 : 128;
+    static constexpr int ROW_BYTES = (HEAVY || NARROW) && !I8 ? 64 : 128;
     static constexpr int STORE_ROWS = store_rows(EPI, F8);   // 32: per-warp stores
     static constexpr int CHUNK_COLS = ROW_BYTES / OUT_BYTES;
     static constexpr int NC = BN / CHUNK_COLS;           // staging chunks per tile
@@ -161,22 +159,23 @@ template <int BN, int EPI, bool PAIR = false, bool F8 = false, bool I8 = false> 
     // issue slots) and for the narrow chunks, two where the chunks are many. The f32 residual stages only
     // acc + bias for its TMA reductions: two groups of one buffer (measured best of 1 x 2, 2 x 1, 2 x 2 and
     // 4 x 1).
-    static constexpr int EG = EPI == kEpiResidual ? ((NC % MF_REDUCE_EG == 0) ? MF_REDUCE_EG : 1)
+    static constexpr int EG = I8 ? (OUT_BYTES == 4 ? 2 : 4) : EPI == kEpiResidual ? ((NC % MF_REDUCE_EG == 0) ? MF_REDUCE_EG : 1)
                               : ((HEAVY || NARROW) && NC % 4 == 0) ? 4 : (NC % 2 == 0 ? 2 : 1);
     // the FP8 bias epilogue with several chunks a group (MF_EPI_BATCH): one staging buffer per chunk, so a group
     // writes all its chunks of a tile before one proxy fence and one barrier, then stores them
     static constexpr bool BATCH = MF_EPI_BATCH && F8_BIAS && NC / EG > 1;
-    static constexpr int NBUF = BATCH ? NC / EG
+    static constexpr int NBUF = I8 ? (OUT_BYTES == 4 ? 2 : 1) : BATCH ? NC / EG
                                 : EPI == kEpiResidual ? MF_REDUCE_NBUF
                                 : F8_BIAS ? MF_F8_BIAS_NBUF : (EG >= 2 ? 1 : 2);   // staging buffers a group
     static constexpr uint32_t A_BYTES = BM * 128;
     static constexpr uint32_t B_BYTES = B_ROWS * 128;
     static constexpr uint32_t STAGE_BYTES = A_BYTES + B_BYTES;
-    static constexpr int STAGES_FIT = (224 * 1024 - EG * NBUF * (int)CHUNK_BYTES) / (int)STAGE_BYTES;
+    static constexpr int VEC_BYTES = I8 ? 2 * 2 * 4 * BN : 0;   // int8: two tiles' column scales and bias
+    static constexpr int STAGES_FIT = (224 * 1024 - EG * NBUF * (int)CHUNK_BYTES - VEC_BYTES) / (int)STAGE_BYTES;
     static constexpr int STAGES = STAGES_FIT > 8 ? 8 : STAGES_FIT;
     static constexpr uint32_t TMEM_COLS = 2 * BN < 32 ? 32 : 2 * BN;
     static constexpr size_t SMEM =
-        1024 + (size_t)STAGES * STAGE_BYTES + (size_t)EG * NBUF * CHUNK_BYTES + 256;
+        1024 + (size_t)STAGES * STAGE_BYTES + (size_t)EG * NBUF * CHUNK_BYTES + VEC_BYTES + 256;
     static constexpr int THREADS = 64 + 128 * EG;
     static_assert(STAGES >= 3, "pipeline too shallow");
     static_assert(SMEM <= 232448, "shared memory over the per-block limit");
@@ -349,39 +348,6 @@ __device__ __forceinline__ float i8_value(int acc, float rowscale, float colscal
     return fmaf(__fmul_rn(__int2float_rn(acc), rowscale), colscale, bias);
 }
 
-// v[i] = i8_value of accumulator r[i] of column col0 + i, i < 32. bias nullptr: 0 (a result of -0 becomes +0 with it).
-__device__ __forceinline__ void scale_i8_32(float (&v)[32], const uint32_t (&r)[32], float rowscale, const EpiArgs& ep,
-                                            int col0, int N)
-{
-    if (col0 + 32 <= N && ep.vec) {
-        const float4* s4 = reinterpret_cast<const float4*>(ep.colscale + col0);
-        const float4* b4 = reinterpret_cast<const float4*>(ep.bias + col0);
-        const uint64_t rs2 = pk2(rowscale, rowscale);
-        const bool has_bias = ep.bias != nullptr;
-#pragma unroll
-        for (int i = 0; i < 8; ++i) {
-            const float4 sc = __ldg(s4 + i);
-            const float4 b = has_bias ? __ldg(b4 + i) : make_float4(0.f, 0.f, 0.f, 0.f);
-            const float2 lo = upk2(fma2(mul2(pk2(__int2float_rn((int)r[4 * i]), __int2float_rn((int)r[4 * i + 1])), rs2),
-                                        pk2(sc.x, sc.y), pk2(b.x, b.y)));
-            const float2 hi =
-                upk2(fma2(mul2(pk2(__int2float_rn((int)r[4 * i + 2]), __int2float_rn((int)r[4 * i + 3])), rs2),
-                          pk2(sc.z, sc.w), pk2(b.z, b.w)));
-            v[4 * i + 0] = lo.x;
-            v[4 * i + 1] = lo.y;
-            v[4 * i + 2] = hi.x;
-            v[4 * i + 3] = hi.y;
-        }
-    } else {
-#pragma unroll
-        for (int i = 0; i < 32; ++i) {
-            const bool in = col0 + i < N;
-            v[i] = i8_value((int)r[i], rowscale, in ? __ldg(ep.colscale + col0 + i) : 0.f,
-                            in && ep.bias ? __ldg(ep.bias + col0 + i) : 0.f);
-        }
-    }
-}
-
 // four floats to four e4m3 bytes (round to nearest even, saturating to +-448), first value in the lowest byte
 __device__ __forceinline__ uint32_t pack_e4m3x4(float a, float b, float c, float d)
 {
@@ -415,7 +381,7 @@ template <typename C> struct SmemLayout {
         sA = smem;
         sB = smem + C::STAGES * C::A_BYTES;
         sC = sB + C::STAGES * C::B_BYTES;                                // EG x NBUF staging chunks
-        full = reinterpret_cast<uint64_t*>(sC + C::EG * C::NBUF * C::CHUNK_BYTES);
+        full = reinterpret_cast<uint64_t*>(sC + C::EG * C::NBUF * C::CHUNK_BYTES + C::VEC_BYTES);
         empty = full + C::STAGES;
         tfull = empty + C::STAGES;
         tempty = tfull + 2;
@@ -455,7 +421,7 @@ __device__ __forceinline__ void epilogue_loop(const SmemLayout<C>& L, const CUte
         if (it < my_tiles && gtid < BN / 32) {
             const int c = origin_col(it) + 32 * gtid;
             if (c < N) {
-                if (!C::IS_I8 || bias) asm volatile("prefetch.global.L1 [%0];" ::"l"(bias + c));
+                asm volatile("prefetch.global.L1 [%0];" ::"l"(bias + c));
                 if constexpr (C::IS_F8) asm volatile("prefetch.global.L1 [%0];" ::"l"(colscale + c));
             }
         }
@@ -467,9 +433,6 @@ __device__ __forceinline__ void epilogue_loop(const SmemLayout<C>& L, const CUte
     int g = 0;        // this group's chunks done
     for (int it = 0; it < my_tiles; ++it) {
         const int row0 = origin_row(it), colb = origin_col(it);
-        float rowscale = 0.f;   // read before the wait for the accumulator, which hides it
-        if constexpr (C::IS_I8)
-            if (row0 + row < M) rowscale = __ldg(ep.rowscale + row0 + row);
         prefetch_bias(it + 1);
         if (leader) L.epi_ok[grp] = mbar_wait(&L.tfull[acc], acc_phase, err, kErrTmemFull) ? 1u : 0u;
         named_barrier(bar_id, 128);
@@ -499,18 +462,15 @@ __device__ __forceinline__ void epilogue_loop(const SmemLayout<C>& L, const CUte
                     if (lane == 0) release(acc);
                 }
                 constexpr int off = 0;
-                if constexpr (!C::IS_I8) {
 #pragma unroll
-                    for (int i = 0; i < 32; ++i) v[off + i] = __uint_as_float(r[i]);
-                }
-                if constexpr (C::IS_I8) scale_i8_32(v, r, rowscale, ep, col0 + 32 * p, N);
-                else if constexpr (C::IS_F8) scale_bias32(v, off, colscale, bias, col0 + 32 * p, N);
+                for (int i = 0; i < 32; ++i) v[off + i] = __uint_as_float(r[i]);
+                if constexpr (C::IS_F8) scale_bias32(v, off, colscale, bias, col0 + 32 * p, N);
                 else add_bias32(v, off, bias, col0 + 32 * p, N);
                 if constexpr (EPI == kEpiBiasGelu) {
                     const GeluK K(1.0f);
 #pragma unroll
                     for (int i = 0; i < 16; ++i) {
-                        const float2 g = gelu_pair<false, C::IS_I8>(pk2(v[2 * i], v[2 * i + 1]), K);
+                        const float2 g = gelu_pair(pk2(v[2 * i], v[2 * i + 1]), K);
                         q[16 * p + i] = pack2<T>(g.x, g.y);
                     }
                 } else if constexpr (EPI == kEpiGeluE4m3) {
@@ -554,29 +514,6 @@ __device__ __forceinline__ void epilogue_loop(const SmemLayout<C>& L, const CUte
                     *reinterpret_cast<uint4*>(buf + swz<RB>(row, j)) =
                         make_uint4(q[4 * j], q[4 * j + 1], q[4 * j + 2], q[4 * j + 3]);
             }
-            if constexpr (C::IS_I8) {
-                if (ep.direct) {
-                    // C does not suit TMA: each warp writes the 32 rows that it staged, a row's columns by its lanes
-                    using TO = std::conditional_t<C::OUT_BYTES == 4, float, T>;
-                    TO* c = static_cast<TO*>(ep.direct);
-                    __syncwarp();
-                    for (int i = 0; i < 32 && row0 + quarter * 32 + i < M; ++i) {
-                        const int rr = quarter * 32 + i;
-                        TO* crow = c + (size_t)(row0 + rr) * ep.ldc;
-#pragma unroll
-                        for (int j = lane; j < C::CHUNK_COLS; j += 32) {
-                            constexpr int PER = 16 / C::OUT_BYTES;   // elements of a 16-byte unit
-                            const TO e = reinterpret_cast<const TO*>(buf + swz<RB>(rr, j / PER))[j % PER];
-                            if (col0 + j < N) {
-                                if constexpr (EPI == kEpiResidual) crow[col0 + j] += e;
-                                else crow[col0 + j] = e;
-                            }
-                        }
-                    }
-                    __syncwarp();   // read, before the next chunk overwrites it
-                    continue;
-                }
-            }
             if (C::BATCH && ci < CPG - 1) continue;   // batched: the fence and the stores after the last chunk
             fence_proxy_async_smem();
             constexpr int NST = C::BATCH ? CPG : 1;   // chunks this fence covers: ci - NST + 1 .. ci
@@ -612,8 +549,127 @@ __device__ __forceinline__ void epilogue_loop(const SmemLayout<C>& L, const CUte
     if (C::STORE_ROWS == 32 ? lane == 0 : leader) bulk_wait_all();
 }
 
+// The epilogue of the int8 products. A warp owns 32 rows of the tile and COLS neighbouring columns of them: it converts
+// them from tensor memory into its own staging chunk of 32 rows x 128 bytes, and its lane 0 stores the chunk (for the
+// residual: adds it at L2) by TMA, so that the warps of a group meet once a tile and not at every chunk. The group's
+// column scales and bias of a tile are read by its 128 threads a tile ahead and passed through shared memory: each is
+// read once from L2, and an aligned float4 serves a warp.
+template <typename TO, int EPI, typename C, typename RowFn, typename ColFn, typename ReleaseFn>
+__device__ __forceinline__ void epilogue_loop_i8(const SmemLayout<C>& L, const CUtensorMap* tmC, uint32_t tmem_base,
+                                                 int my_tiles, RowFn origin_row, ColFn origin_col, ReleaseFn release,
+                                                 const EpiArgs& ep, int M, int N, uint32_t* err)
+{
+    griddep_wait();
+    constexpr int COLS = C::BN / C::EG;               // columns of a group
+    constexpr int VECS = 2 * COLS;                    // its column scales, then its bias
+    constexpr int PER = VECS / 128;
+    constexpr int CHUNK = C::CHUNK_COLS;              // columns of 128 bytes
+    static_assert(VECS % 128 == 0 && COLS % CHUNK == 0 && C::ROW_BYTES == 128, "a group's columns must be whole chunks");
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    const int grp = (warp - 2) >> 2, gtid = (int)threadIdx.x - 64 - 128 * grp;
+    const int quarter = warp & 3;
+    const int row = quarter * 32 + lane;
+    const uint32_t bar_id = 1 + grp;
+    const uint32_t t_lane = tmem_base + (static_cast<uint32_t>(quarter * 32) << 16) + static_cast<uint32_t>(grp * COLS);
+    uint8_t* const stages = L.sC + (grp * 4 + quarter) * C::NBUF * 4096;
+    float* const svec = reinterpret_cast<float*>(L.sC + C::EG * C::NBUF * C::CHUNK_BYTES) + grp * 2 * VECS;
+    int chunk = 0;
+
+    float next[PER], next_rs = 0.f;
+    auto read_ahead = [&](int it) {
+        if (it >= my_tiles) return;
+        const int col0 = origin_col(it) + grp * COLS, r = origin_row(it) + row;
+#pragma unroll
+        for (int j = 0; j < PER; ++j) {
+            const int k = gtid + 128 * j, n = col0 + (k & (COLS - 1));
+            const float* src = k < COLS ? ep.colscale : ep.bias;
+            next[j] = src && n < N ? __ldg(src + n) : 0.f;
+        }
+        next_rs = r < M ? __ldg(ep.rowscale + r) : 0.f;
+    };
+    read_ahead(0);
+
+    int acc = 0;
+    uint32_t acc_phase = 0;
+    for (int it = 0; it < my_tiles; ++it) {
+        const int row0 = origin_row(it) + quarter * 32, col0 = origin_col(it) + grp * COLS;
+        float* sv = svec + (it & 1) * VECS;           // the other half is still read by this group's slower warps
+#pragma unroll
+        for (int j = 0; j < PER; ++j) sv[gtid + 128 * j] = next[j];
+        const uint64_t rs2 = pk2(next_rs, next_rs);
+        if (gtid == 0) L.epi_ok[grp] = mbar_wait(&L.tfull[acc], acc_phase, err, kErrTmemFull) ? 1u : 0u;
+        named_barrier(bar_id, 128);
+        if (!L.epi_ok[grp]) break;
+        tc_fence_after();
+        read_ahead(it + 1);
+        const uint32_t t_acc = t_lane + static_cast<uint32_t>(acc * C::BN);
+#pragma unroll 1
+        for (int c = 0; c < COLS; c += CHUNK) {
+            uint32_t q[32];                            // the row's 128 bytes
+#pragma unroll
+            for (int p = 0; p < CHUNK; p += 32) {
+                uint32_t a[32];
+                tmem_ld_32x32b_x32(t_acc + static_cast<uint32_t>(c + p), a);
+                tmem_ld_wait();
+                if (c + p == COLS - 32) {
+                    tc_fence_before();
+                    __syncwarp();
+                    if (lane == 0) release(acc);
+                }
+#pragma unroll
+                for (int i = 0; i < 32; i += 4) {
+                    const float4 sc = *reinterpret_cast<const float4*>(sv + c + p + i);
+                    const float4 b = *reinterpret_cast<const float4*>(sv + COLS + c + p + i);
+                    const uint64_t lo = fma2(mul2(pk2(__int2float_rn((int)a[i]), __int2float_rn((int)a[i + 1])), rs2),
+                                             pk2(sc.x, sc.y), pk2(b.x, b.y));
+                    const uint64_t hi =
+                        fma2(mul2(pk2(__int2float_rn((int)a[i + 2]), __int2float_rn((int)a[i + 3])), rs2),
+                             pk2(sc.z, sc.w), pk2(b.z, b.w));
+                    float2 x, y;
+                    if constexpr (EPI == kEpiBiasGelu) {
+                        const GeluK K(1.0f);
+                        x = gelu_pair<false, true>(lo, K);
+                        y = gelu_pair<false, true>(hi, K);
+                    } else {
+                        x = upk2(lo);
+                        y = upk2(hi);
+                    }
+                    if constexpr (sizeof(TO) == 2) {
+                        q[(p + i) / 2] = pack2<TO>(x.x, x.y);
+                        q[(p + i) / 2 + 1] = pack2<TO>(y.x, y.y);
+                    } else {
+                        q[i] = __float_as_uint(x.x);
+                        q[i + 1] = __float_as_uint(x.y);
+                        q[i + 2] = __float_as_uint(y.x);
+                        q[i + 3] = __float_as_uint(y.y);
+                    }
+                }
+            }
+            uint8_t* stage = stages + (chunk % C::NBUF) * 4096;
+            ++chunk;
+            if (lane == 0) bulk_wait_read<C::NBUF - 1>();   // the last store out of this chunk has read it
+            __syncwarp();
+#pragma unroll
+            for (int j = 0; j < 8; ++j)
+                *reinterpret_cast<uint4*>(stage + swz<128>(lane, j)) =
+                    make_uint4(q[4 * j], q[4 * j + 1], q[4 * j + 2], q[4 * j + 3]);
+            fence_proxy_async_smem();
+            __syncwarp();
+            if (lane == 0 && row0 < M) {
+                if constexpr (EPI == kEpiResidual) tma_reduce_add_2d(tmC, stage, col0 + c, row0);
+                else tma_store_2d(tmC, stage, col0 + c, row0);
+                bulk_commit();
+            }
+        }
+        acc ^= 1;
+        if (acc == 0) acc_phase ^= 1u;
+    }
+    if (lane == 0) bulk_wait_all();
+}
+
 // ------------------------------------------------------------------------------------------------ one CTA
-// TI: the operands' type (f16, bf16 or e4m3); T: the 16-bit output type of kEpiBias / kEpiBiasGelu.
+// TI: the operands' type (f16, bf16, e4m3 or int8); T: the 16-bit output type of kEpiBias / kEpiBiasGelu (int8: the
+// output's type, f32 among them).
 template <typename TI, typename T, int BN, int EPI>
 __global__ void __launch_bounds__(GemmCfg<BN, EPI, false, Operand<TI>::F8, Operand<TI>::I8>::THREADS, 1)
 gemm_tc_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant__ CUtensorMap tmB,
@@ -739,14 +795,16 @@ gemm_tc_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant__ 
     } else if (k_iters > 0) {
         const int my_tiles =
             (int)blockIdx.x < num_tiles ? (num_tiles - 1 - (int)blockIdx.x) / (int)gridDim.x + 1 : 0;
-        epilogue_loop<T, EPI, C>(
-            L, &tmC, tmem_base, my_tiles,
-            [&](int it) {
-                const int m_fwd = ((int)blockIdx.x + it * (int)gridDim.x) / n_tiles;
-                return (ep.rev ? m_tiles - 1 - m_fwd : m_fwd) * C::BM;
-            },
-            [&](int it) { return (((int)blockIdx.x + it * (int)gridDim.x) % n_tiles) * BN; },
-            [&](int acc) { mbar_arrive(&L.tempty[acc]); }, ep, M, N, err);
+        const auto origin_row = [&](int it) {
+            const int m_fwd = ((int)blockIdx.x + it * (int)gridDim.x) / n_tiles;
+            return (ep.rev ? m_tiles - 1 - m_fwd : m_fwd) * C::BM;
+        };
+        const auto origin_col = [&](int it) { return (((int)blockIdx.x + it * (int)gridDim.x) % n_tiles) * BN; };
+        const auto release = [&](int acc) { mbar_arrive(&L.tempty[acc]); };
+        if constexpr (C::IS_I8)
+            epilogue_loop_i8<T, EPI, C>(L, &tmC, tmem_base, my_tiles, origin_row, origin_col, release, ep, M, N, err);
+        else
+            epilogue_loop<T, EPI, C>(L, &tmC, tmem_base, my_tiles, origin_row, origin_col, release, ep, M, N, err);
     }
 
     __syncwarp();
@@ -899,14 +957,20 @@ gemm_tc_pair_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_consta
         const int my_tiles = pair < num_tiles ? (num_tiles - 1 - pair) / num_pairs + 1 : 0;
         const uint32_t tempty_lead0 = mapa_shared(smem_u32(&L.tempty[0]), 0);
         const uint32_t tempty_lead1 = mapa_shared(smem_u32(&L.tempty[1]), 0);
-        epilogue_loop<T, EPI, C>(
-            L, &tmC, tmem_base, my_tiles,
-            [&](int it) {
-                const int m_fwd = (pair + it * num_pairs) / n_tiles;
-                return (ep.rev ? m_tiles - 1 - m_fwd : m_fwd) * 2 * C::BM + (int)rank * C::BM;
-            },
-            [&](int it) { return ((pair + it * num_pairs) % n_tiles) * BN; },
-            [&](int acc) { mbar_arrive_cluster(acc ? tempty_lead1 : tempty_lead0); }, ep, M, N, err);
+        const auto origin_row = [&](int it) {
+            const int m_fwd = (pair + it * num_pairs) / n_tiles;
+            return (ep.rev ? m_tiles - 1 - m_fwd : m_fwd) * 2 * C::BM + (int)rank * C::BM;
+        };
+        const auto origin_col = [&](int it) { return ((pair + it * num_pairs) % n_tiles) * BN; };
+        const auto release = [&](int acc) {
+            const uint32_t bar = acc ? tempty_lead1 : tempty_lead0;
+            if constexpr (C::IS_I8) mbar_arrive_cluster_tmem(bar);
+            else mbar_arrive_cluster(bar);
+        };
+        if constexpr (C::IS_I8)
+            epilogue_loop_i8<T, EPI, C>(L, &tmC, tmem_base, my_tiles, origin_row, origin_col, release, ep, M, N, err);
+        else
+            epilogue_loop<T, EPI, C>(L, &tmC, tmem_base, my_tiles, origin_row, origin_col, release, ep, M, N, err);
     }
 
     __syncwarp();

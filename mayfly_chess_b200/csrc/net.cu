@@ -1723,28 +1723,32 @@ static int pick_i8_kernel(const GemmI8& p, int num_sms)
 template <typename TO, int EPI>
 static void launch_gemm_i8_t(const GemmI8& p, int kernel, cudaStream_t s)
 {
-    using T = std::conditional_t<std::is_same<TO, float>::value, __nv_bfloat16, TO>;   // not used by f32 outputs
     int dev = 0, sms = 0;
     RT(cudaGetDevice(&dev));
     RT(cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, dev));
+    // a TMA store writes whole 16-byte units, the last of a row past its end too: rows must be made of such units
+    const bool units = reinterpret_cast<uintptr_t>(p.C) % 16 == 0 && p.N * sizeof(TO) % 16 == 0 &&
+                       (p.M == 1 || p.ldc * sizeof(TO) % 16 == 0);
+    if (!units) {
+        launch_k(gemm_i8_simple_kernel<TO, EPI>, dim3((p.N + 15) / 16, (p.M + 15) / 16), dim3(256), 0, s,
+                 static_cast<const int8_t*>(p.A), static_cast<const int8_t*>(p.W), p.rowscale, p.colscale, p.bias,
+                 static_cast<TO*>(p.C), p.M, p.N, p.K, p.lda, p.ldw, p.ldc);
+        return;
+    }
     if (kernel < 0) kernel = pick_i8_kernel(p, sms);
     const auto pitch = [](long long ld, int width, int rows) { return rows > 1 ? ld : (width + 15LL) / 16 * 16; };
     const CUtensorMap ma = make_map(p.A, MapType::U8, p.K, p.M, pitch(p.lda, p.K, p.M), 128, 128);
     const CUtensorMap mb = make_map(p.W, MapType::U8, p.K, p.N, pitch(p.ldw, p.K, p.N), 128,
                                     w_box_rows(kernel == kI8Pair ? kPairTile : 256));
-    // a TMA store writes whole 16-byte units, the last of a row past its end too: rows must be made of such units
-    const bool tma_out = reinterpret_cast<uintptr_t>(p.C) % 16 == 0 && p.N * sizeof(TO) % 16 == 0 &&
-                         (p.M == 1 || p.ldc * sizeof(TO) % 16 == 0);
-    // with direct stores the kernel never uses the output's map: any valid one
-    const CUtensorMap mc = tma_out ? output_map(p.C, EPI, type16(std::is_same<T, __nv_bfloat16>::value), p.M, p.N,
-                                                pitch(p.ldc, p.N, p.M), true)
-                                   : ma;
-    const auto low = reinterpret_cast<uintptr_t>(p.colscale) | reinterpret_cast<uintptr_t>(p.bias);
-    const EpiArgs ep{p.bias, p.colscale, 1.f, 0, p.rowscale, tma_out ? nullptr : p.C, p.ldc, low % 16 == 0};
+    constexpr MapType t = std::is_same<TO, float>::value    ? MapType::F32
+                          : std::is_same<TO, __half>::value ? MapType::F16
+                                                            : MapType::BF16;
+    const CUtensorMap mc = make_map(p.C, t, p.N, p.M, p.M > 1 ? p.ldc : (p.N + 15LL) / 16 * 16, 128 / sizeof(TO), 32);
+    const EpiArgs ep{p.bias, p.colscale, 1.f, 0, p.rowscale};
     if (kernel == kI8Pair)
-        launch_gemm_pair<int8_t, T, EPI>(ma, mb, mc, p.M, p.N, p.K, ep, i8_error_word(dev), s);
+        launch_gemm_pair<int8_t, TO, EPI>(ma, mb, mc, p.M, p.N, p.K, ep, i8_error_word(dev), s);
     else
-        launch_gemm_bn<int8_t, T, 256, EPI>(ma, mb, mc, p.M, p.N, p.K, ep, i8_error_word(dev), sms, s);
+        launch_gemm_bn<int8_t, TO, 256, EPI>(ma, mb, mc, p.M, p.N, p.K, ep, i8_error_word(dev), sms, s);
 }
 
 // A null pointer, or one whose address is no multiple of `align`, named in the reason.

@@ -275,6 +275,13 @@ __device__ __forceinline__ void mbar_arrive_cluster(uint32_t cluster_addr)
     asm volatile("mbarrier.arrive.release.cluster.shared::cluster.b64 _, [%0];" ::"r"(cluster_addr) : "memory");
 }
 
+// the same with release at CTA scope: the arrival does not wait for this thread's earlier global writes to reach the
+// cluster. For handing over tensor memory only, whose accesses tcgen05.fence and tcgen05.wait order.
+__device__ __forceinline__ void mbar_arrive_cluster_tmem(uint32_t cluster_addr)
+{
+    asm volatile("mbarrier.arrive.release.cta.shared::cluster.b64 _, [%0];" ::"r"(cluster_addr) : "memory");
+}
+
 // TMA tile load into this CTA's shared memory whose completion is counted on a barrier of either CTA of the
 // pair (here always the leader's); no multicast.
 __device__ __forceinline__ void tma_load_2d_pair(void* dst, const CUtensorMap* map, uint32_t bar_cluster_addr, int x,

@@ -585,78 +585,82 @@ def k_layernorm_f8(x, g, b, h, n, d, mul, row_stride=1, dll=None):
 
 
 # ------------------------------------------------------------------------------------------------ int8 operators
-# These calls queue one kernel and return, so what a call costs on the host is most of what a small one costs: the
-# checks read each tensor's attributes once, and the reason buffer is kept per thread.
-_i8_local = threading.local()
-_i8_types = {}
+# These calls queue one kernel and return, so what a call costs on the host is most of what a small one costs (the
+# library's part is about 3.5 us, the launch among it). Hence one straight line of checks that reads each attribute
+# once, the torch objects and the default library looked up once a process, and a reason buffer kept by each thread.
+class _I8(threading.local):
+    def __init__(self):
+        self.reason = ctypes.create_string_buffer(ERR_LEN)
 
 
-def _i8_reason():
-    try:
-        return _i8_local.reason
-    except AttributeError:
-        _i8_local.reason = ctypes.create_string_buffer(ERR_LEN)
-        return _i8_local.reason
+_i8_local = _I8()
+_i8_once = None
 
 
-def _i8_type(t, name):
-    """The C ABI's code of a tensor's element type: 0 f16, 1 bf16, 2 f32."""
-    if not _i8_types:
+class _I8Once:
+    """What the int8 calls need of torch: dtypes, their codes in the C ABI, the current device and stream."""
+
+    def __init__(self):
         import torch
-        _i8_types.update({torch.float16: 0, torch.bfloat16: 1, torch.float32: 2})
-    code = _i8_types.get(t.dtype)
-    if code is None:
-        raise ValueError(f"{name}: float16, bfloat16 or float32 only, got {t.dtype}")
-    return code
+        self.int8, self.f32 = torch.int8, torch.float32
+        self.types = {torch.float16: 0, torch.bfloat16: 1, torch.float32: 2}
+        self.on_device = torch.cuda.device
+        # what torch's own generated code calls: a tenth of the cost of building a Stream object
+        self.device = getattr(torch._C, "_cuda_getDevice", None) or torch.cuda.current_device
+        self.stream = (getattr(torch._C, "_cuda_getCurrentRawStream", None)
+                       or (lambda dev: torch.cuda.current_stream(dev).cuda_stream))
+        self.lib = None
+
+    def load(self, dll):
+        """The library of `dll`; the default one (MAYFLY_CUDANET_DLL, else this package's) is looked up once."""
+        if dll is not None:
+            return load(dll)
+        if self.lib is None:
+            self.lib = load()
+        return self.lib
 
 
-def _i8_codes(t, name):
-    import torch
-    if t.dtype != torch.int8:
-        raise ValueError(f"{name}: int8 only, got {t.dtype}")
+def _i8_setup():
+    global _i8_once
+    if _i8_once is None:
+        _i8_once = _I8Once()
+    return _i8_once
 
 
-def _i8_vec(t, name, n, dev):
-    """A contiguous float32 vector of n elements on device index dev; its address."""
-    if _i8_type(t, name) != 2:
-        raise ValueError(f"{name}: float32 only, got {t.dtype}")
-    if t.shape != (n,) or (n > 1 and t.stride(0) != 1):
-        raise ValueError(f"{name}: shape {tuple(t.shape)} strides {t.stride()}, expected ({n},) contiguous")
-    if t.get_device() != dev:
-        raise ValueError(f"{name}: on {t.device}, expected cuda:{dev}")
-    return t.data_ptr()
+def _i8_bad_type(name, t, want):
+    return ValueError(f"{name}: {want} only, got {t.dtype}")
 
 
-def _i8_mat(t, name, shape, dev):
-    """The row pitch of a matrix whose rows are contiguous, after the checks of its shape and device."""
+def _i8_rows(t, name, shape, dev):
+    """The row pitch of a matrix of this shape on device index dev, its rows contiguous."""
     if t.shape != shape:
         raise ValueError(f"{name}: shape {tuple(t.shape)}, expected {tuple(shape)}")
-    if t.get_device() != dev:
-        raise ValueError(f"{name}: on {t.device}, expected cuda:{dev}")
+    if t.get_device() != dev or dev < 0:
+        raise ValueError(f"{name}: on {t.device}, expected a tensor of one CUDA device with the others")
     pitch, step = t.stride()
     if step != 1 and shape[1] > 1:
         raise ValueError(f"{name}: rows must be contiguous, got strides {t.stride()}")
     return pitch
 
 
-def _i8_device(t, name):
-    """The index of the CUDA device a 2-d tensor is on."""
-    if t.dim() != 2:
-        raise ValueError(f"{name}: shape {tuple(t.shape)}, expected a matrix")
-    dev = t.get_device()
-    if dev < 0:
-        raise ValueError(f"{name}: needs a CUDA tensor, got one on {t.device}")
-    return dev
+def _i8_vec(t, name, n, dev, f32):
+    """The address of a contiguous float32 vector of n elements on device index dev."""
+    if t.dtype is not f32:
+        raise _i8_bad_type(name, t, "float32")
+    if t.shape != (n,) or not t.is_contiguous():
+        raise ValueError(f"{name}: shape {tuple(t.shape)} strides {t.stride()}, expected ({n},) contiguous")
+    if t.get_device() != dev:
+        raise ValueError(f"{name}: on {t.device}, expected a tensor of one CUDA device with the others")
+    return t.data_ptr()
 
 
-def _i8_call(fn, dev, *args):
+def _i8_call(once, fn, dev, *args):
     """fn(*args, stream, reason) on device `dev` and its current stream; RuntimeError with the library's reason."""
-    import torch
-    if torch.cuda.current_device() != dev:
-        with torch.cuda.device(dev):
-            return _i8_call(fn, dev, *args)
-    reason = _i8_reason()
-    if fn(*args, torch.cuda.current_stream(dev).cuda_stream, reason, ERR_LEN) != 0:
+    if once.device() != dev:
+        with once.on_device(dev):
+            return _i8_call(once, fn, dev, *args)
+    reason = _i8_local.reason
+    if fn(*args, once.stream(dev), reason, ERR_LEN) != 0:
         raise RuntimeError(f"{fn.__name__}: {_msg(reason)}")
 
 
@@ -666,25 +670,34 @@ def k_rmsnorm_i8(x, delta, g, out, q, scale, eps=1e-6, dll=None):
     of any of the three where x is float32; out may be x (in place). delta and out None: the norm of x alone. q (M, D)
     int8, scale (M,) float32. Rows may have any pitch; asynchronous on the device's current stream. Returns (q,
     scale)."""
-    lib = load(dll)
-    dev = _i8_device(x, "x")
-    shape = x.shape
+    once = _i8_once or _i8_setup()
+    xt = once.types.get(x.dtype)
+    if xt is None:
+        raise _i8_bad_type("x", x, "float16, bfloat16 or float32")
+    if q.dtype is not once.int8:
+        raise _i8_bad_type("q", q, "int8")
+    shape, dev = x.shape, x.get_device()
+    if len(shape) != 2:
+        raise ValueError(f"x: shape {tuple(shape)}, expected a matrix")
     M, D = shape
-    xt = _i8_type(x, "x")
-    ldx, ldq = _i8_mat(x, "x", shape, dev), _i8_mat(q, "q", shape, dev)
-    _i8_codes(q, "q")
-    gp, sp = _i8_vec(g, "g", D, dev), _i8_vec(scale, "scale", M, dev)
-    if (delta is None) != (out is None):
-        raise ValueError("delta and out: both or neither (out holds the sum)")
+    ldx, ldq = _i8_rows(x, "x", shape, dev), _i8_rows(q, "q", shape, dev)
     if delta is None:
+        if out is not None:
+            raise ValueError("out without delta: there is no sum to store")
         dt, ldd, ldo, dp, op = xt, 0, 0, None, None
     else:
-        dt, ldd, ldo = _i8_type(delta, "delta"), _i8_mat(delta, "delta", shape, dev), _i8_mat(out, "out", shape, dev)
-        if out.dtype != x.dtype:
-            raise ValueError(f"out: {x.dtype} as x, got {out.dtype}")
+        dt = once.types.get(delta.dtype)
+        if dt is None:
+            raise _i8_bad_type("delta", delta, "float16, bfloat16 or float32")
+        if out is None:
+            raise ValueError("delta without out: out holds the sum (x itself: in place)")
+        if out.dtype is not x.dtype:
+            raise _i8_bad_type("out", out, f"x's {x.dtype}")
+        ldd, ldo = _i8_rows(delta, "delta", shape, dev), ldx if out is x else _i8_rows(out, "out", shape, dev)
         dp, op = delta.data_ptr(), out.data_ptr()
-    _i8_call(lib.cudanet_k_rmsnorm_i8, dev, xt, dt, x.data_ptr(), dp, gp, op, q.data_ptr(), sp, M, D, ldx, ldd, ldo,
-             ldq, eps)
+    _i8_call(once, once.load(dll).cudanet_k_rmsnorm_i8, dev, xt, dt, x.data_ptr(), dp,
+             _i8_vec(g, "g", D, dev, once.f32), op, q.data_ptr(), _i8_vec(scale, "scale", M, dev, once.f32), M, D, ldx,
+             ldd, ldo, ldq, eps)
     return q, scale
 
 
@@ -692,14 +705,19 @@ def k_quant_i8(x, q, scale, dll=None):
     """x (M, D) float32, bfloat16 or float16 as int8 rows with a float32 scale each: scale = max |row| / 127, q * scale
     stands for x. A weight matrix (N, K) gets a scale for each output channel. Rows may have any pitch; asynchronous on
     the device's current stream. Returns (q, scale)."""
-    lib = load(dll)
-    dev = _i8_device(x, "x")
-    shape = x.shape
+    once = _i8_once or _i8_setup()
+    xt = once.types.get(x.dtype)
+    if xt is None:
+        raise _i8_bad_type("x", x, "float16, bfloat16 or float32")
+    if q.dtype is not once.int8:
+        raise _i8_bad_type("q", q, "int8")
+    shape, dev = x.shape, x.get_device()
+    if len(shape) != 2:
+        raise ValueError(f"x: shape {tuple(shape)}, expected a matrix")
     M, D = shape
-    ldx, ldq = _i8_mat(x, "x", shape, dev), _i8_mat(q, "q", shape, dev)
-    _i8_codes(q, "q")
-    _i8_call(lib.cudanet_k_quant_i8, dev, _i8_type(x, "x"), x.data_ptr(), q.data_ptr(), _i8_vec(scale, "scale", M, dev),
-             M, D, ldx, ldq)
+    ldx, ldq = _i8_rows(x, "x", shape, dev), _i8_rows(q, "q", shape, dev)
+    _i8_call(once, once.load(dll).cudanet_k_quant_i8, dev, xt, x.data_ptr(), q.data_ptr(),
+             _i8_vec(scale, "scale", M, dev, once.f32), M, D, ldx, ldq)
     return q, scale
 
 
@@ -707,19 +725,23 @@ def k_gemm_i8(A, W, rowscale, colscale, bias, C, epi, kernel=-1, dll=None):
     """C = epilogue(A W^T * rowscale[m] * colscale[n] + bias[n]) with int8 A (M, K) and W (N, K), whose rows begin on
     16 bytes, the sum exact in int32, rowscale (M,), colscale (N,) and bias (N,) or None float32: epi 0 16-bit out, 1
     GELU and 16-bit out, 2 C += (float32), 3 float32 out. Asynchronous on the device's current stream. Returns C."""
-    lib = load(dll)
-    dev = _i8_device(A, "A")
-    _i8_codes(A, "A")
-    _i8_codes(W, "W")
-    M, K = A.shape
-    N = W.shape[0]
-    lda, ldw, ldc = _i8_mat(A, "A", (M, K), dev), _i8_mat(W, "W", (N, K), dev), _i8_mat(C, "C", (M, N), dev)
-    ct = _i8_type(C, "C")
-    if (ct == 2) != (epi >= 2):
-        raise ValueError(f"C: epi {epi} writes {'float32' if epi >= 2 else '16-bit floats'}, got {C.dtype}")
-    _i8_call(lib.cudanet_k_gemm_i8, dev, ct & 1, epi, kernel, A.data_ptr(), W.data_ptr(),
-             _i8_vec(rowscale, "rowscale", M, dev), _i8_vec(colscale, "colscale", N, dev),
-             None if bias is None else _i8_vec(bias, "bias", N, dev), C.data_ptr(), M, N, K, lda, ldw, ldc)
+    once = _i8_once or _i8_setup()
+    if A.dtype is not once.int8:
+        raise _i8_bad_type("A", A, "int8")
+    if W.dtype is not once.int8:
+        raise _i8_bad_type("W", W, "int8")
+    ct = once.types.get(C.dtype)
+    if ct is None or (ct == 2) != (epi >= 2):
+        raise _i8_bad_type("C", C, f"epi {epi} writes float32: it" if epi >= 2 else "float16 or bfloat16")
+    sa, sw, dev = A.shape, W.shape, A.get_device()
+    if len(sa) != 2 or len(sw) != 2 or sa[1] != sw[1]:
+        raise ValueError(f"A and W: shapes {tuple(sa)} and {tuple(sw)}, expected (M, K) and (N, K)")
+    M, K = sa
+    N = sw[0]
+    lda, ldw, ldc = _i8_rows(A, "A", sa, dev), _i8_rows(W, "W", sw, dev), _i8_rows(C, "C", (M, N), dev)
+    _i8_call(once, once.load(dll).cudanet_k_gemm_i8, dev, ct & 1, epi, kernel, A.data_ptr(), W.data_ptr(),
+             _i8_vec(rowscale, "rowscale", M, dev, once.f32), _i8_vec(colscale, "colscale", N, dev, once.f32),
+             None if bias is None else _i8_vec(bias, "bias", N, dev, once.f32), C.data_ptr(), M, N, K, lda, ldw, ldc)
     return C
 
 
