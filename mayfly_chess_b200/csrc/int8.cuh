@@ -15,7 +15,7 @@
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
 
-#include "gemm.cuh"
+#include "trunk.cuh"
 
 namespace mf {
 
@@ -42,53 +42,164 @@ __device__ __forceinline__ RowScale row_scale(uint32_t amax_bits, float r)
     return {__fdiv_rn(a * r, 127.f), __fdiv_rn(127.f, a)};
 }
 
-// The code of t. A row without a scale (inv 0) has codes 0, whatever t is.
-__device__ __forceinline__ int code_of(float t, float inv) { return inv == 0.f ? 0 : __float2int_rn(t * inv); }
+// The arguments of the row kernels (pitches in elements). delta and out nullptr: nothing is added or stored.
+struct RowsI8 {
+    const void *x, *delta;
+    const float* g;          // the norm only
+    void* out;
+    int8_t* q;
+    float* scale;
+    int M, D;
+    long long ldx, ldd, ldo, ldq;
+    float eps;
+};
 
-// One block a row; D any, every element by itself.
-template <typename XT, typename DT, bool NORM>
-__global__ void __launch_bounds__(256) rows_i8_kernel(const XT* __restrict__ x, const DT* __restrict__ delta,
-                                                      const float* __restrict__ g, XT* out, int8_t* __restrict__ q,
-                                                      float* __restrict__ scale, int D, long long ldx, long long ldd,
-                                                      long long ldo, long long ldq, float eps)
+// 8 neighbouring elements from an address on 16 bytes
+__device__ __forceinline__ void load8(const float* p, float (&v)[8])
+{
+    const float4 a = __ldg(reinterpret_cast<const float4*>(p)), b = __ldg(reinterpret_cast<const float4*>(p) + 1);
+    v[0] = a.x, v[1] = a.y, v[2] = a.z, v[3] = a.w, v[4] = b.x, v[5] = b.y, v[6] = b.z, v[7] = b.w;
+}
+__device__ __forceinline__ void load8(const __nv_bfloat16* p, float (&v)[8])
+{
+    const uint4 a = __ldg(reinterpret_cast<const uint4*>(p));
+    const uint32_t w[4] = {a.x, a.y, a.z, a.w};
+#pragma unroll
+    for (int i = 0; i < 4; ++i) v[2 * i] = bf16_lo(w[i]), v[2 * i + 1] = bf16_hi(w[i]);
+}
+__device__ __forceinline__ void load8(const __half* p, float (&v)[8])
+{
+    const uint4 a = __ldg(reinterpret_cast<const uint4*>(p));
+    const uint32_t w[4] = {a.x, a.y, a.z, a.w};
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+        const float2 f = __half22float2(*reinterpret_cast<const __half2*>(&w[i]));
+        v[2 * i] = f.x, v[2 * i + 1] = f.y;
+    }
+}
+__device__ __forceinline__ void store8(float* p, const float (&v)[8])
+{
+    reinterpret_cast<float4*>(p)[0] = make_float4(v[0], v[1], v[2], v[3]);
+    reinterpret_cast<float4*>(p)[1] = make_float4(v[4], v[5], v[6], v[7]);
+}
+template <typename T> __device__ __forceinline__ void store8(T* p, const float (&v)[8])
+{
+    *reinterpret_cast<uint4*>(p) =
+        make_uint4(pack2<T>(v[0], v[1]), pack2<T>(v[2], v[3]), pack2<T>(v[4], v[5]), pack2<T>(v[6], v[7]));
+}
+
+// The code of t as the low byte of t * inv + 1.5 * 2^23, whose sum is rounded to a whole number, ties to even: one
+// instruction where a conversion to an integer runs at a quarter of the rate. |t * inv| < 127.001.
+__device__ __forceinline__ uint32_t code_byte(float t, float inv) { return __float_as_uint(fmaf(t, inv, 12582912.f)); }
+__device__ __forceinline__ uint32_t codes4(float a, float b, float c, float d, float inv)
+{
+    return __byte_perm(__byte_perm(code_byte(a, inv), code_byte(b, inv), 0x0040),
+                       __byte_perm(code_byte(c, inv), code_byte(d, inv), 0x0040), 0x5410);
+}
+
+// T threads hold a row in registers (a warp each, T = 32, or a block), 8 V elements a thread, so x and delta are read
+// and out, q and scale written once: bound by HBM from about a thousand rows. VEC: neighbouring elements 8 at a time
+// (every row of every operand begins on 16 bytes, q's on 8); else element by element, T apart.
+template <typename XT, typename DT, bool NORM, bool VEC, int T, int V>
+__global__ void __launch_bounds__(T == 32 ? 256 : T) rows_i8_kernel(const RowsI8 a)
 {
     griddep_wait();
     griddep_launch();
-    __shared__ float s_sum[8];
-    __shared__ uint32_t s_max[8];
-    const size_t row = blockIdx.x;
-    auto value = [&](int i) {
-        float s = to_f32(x[row * ldx + i]);
-        if (delta) s = to_f32(from_f32<XT>(s + to_f32(delta[row * ldd + i])));
-        return s;
-    };
+    const int t = T == 32 ? threadIdx.x & 31 : threadIdx.x;
+    const size_t row = T == 32 ? (size_t)blockIdx.x * (blockDim.x >> 5) + (threadIdx.x >> 5) : blockIdx.x;
+    if (row >= (size_t)a.M) return;   // T = 32: a whole warp
+    const XT* __restrict__ x = static_cast<const XT*>(a.x) + row * a.ldx;
+    const DT* __restrict__ delta = static_cast<const DT*>(a.delta) + row * a.ldd;
+    XT* out = static_cast<XT*>(a.out) + row * a.ldo;
+    int8_t* q = a.q + row * a.ldq;
+    const bool add = NORM && a.delta;
+    const int D = a.D;
+    // element j of vector v of this thread; VEC: the last vector of the row may be cut
+    auto at = [&](int v, int j) { return VEC ? 8 * (t + T * v) + j : t + T * (8 * v + j); };
+    auto whole = [&](int v) { return VEC && at(v, 8) <= D; };
+
+    float s[V][8];
+#pragma unroll
+    for (int v = 0; v < V; ++v) {
+        if (whole(v)) load8(x + at(v, 0), s[v]);
+        else {
+#pragma unroll
+            for (int j = 0; j < 8; ++j) s[v][j] = at(v, j) < D ? to_f32(x[at(v, j)]) : 0.f;
+        }
+    }
+    if (add) {
+        float d[V][8];
+#pragma unroll
+        for (int v = 0; v < V; ++v) {
+            if (whole(v)) load8(delta + at(v, 0), d[v]);
+            else {
+#pragma unroll
+                for (int j = 0; j < 8; ++j) d[v][j] = at(v, j) < D ? to_f32(delta[at(v, j)]) : 0.f;
+            }
+        }
+#pragma unroll
+        for (int v = 0; v < V; ++v) {
+#pragma unroll
+            for (int j = 0; j < 8; ++j) s[v][j] = to_f32(from_f32<XT>(s[v][j] + d[v][j]));
+            if (whole(v)) store8(out + at(v, 0), s[v]);
+            else {
+#pragma unroll
+                for (int j = 0; j < 8; ++j)
+                    if (at(v, j) < D) out[at(v, j)] = from_f32<XT>(s[v][j]);
+            }
+        }
+    }
     float ss = 0.f;
     uint32_t mx = 0;
-    for (int i = threadIdx.x; i < D; i += 256) {
-        const float s = value(i);
-        ss += s * s;
-        mx = max(mx, __float_as_uint(NORM ? s * g[i] : s) & 0x7FFFFFFFu);
+#pragma unroll
+    for (int v = 0; v < V; ++v) {
+        if constexpr (NORM) {
+            float g[8];
+            if (whole(v)) load8(a.g + at(v, 0), g);
+            else {
+#pragma unroll
+                for (int j = 0; j < 8; ++j) g[j] = at(v, j) < D ? __ldg(a.g + at(v, j)) : 0.f;
+            }
+#pragma unroll
+            for (int j = 0; j < 8; ++j) {
+                ss = fmaf(s[v][j], s[v][j], ss);
+                s[v][j] *= g[j];
+            }
+        }
+#pragma unroll
+        for (int j = 0; j < 8; ++j) mx = max(mx, __float_as_uint(s[v][j]) & 0x7FFFFFFFu);
     }
-    for (int o = 16; o > 0; o >>= 1) ss += __shfl_xor_sync(0xffffffffu, ss, o);
+    if constexpr (NORM) ss = warp_sum(ss);
     mx = __reduce_max_sync(0xffffffffu, mx);
-    if ((threadIdx.x & 31) == 0) {
-        s_sum[threadIdx.x >> 5] = ss;
-        s_max[threadIdx.x >> 5] = mx;
+    if constexpr (T > 32) {
+        __shared__ float s_sum[T / 32];
+        __shared__ uint32_t s_max[T / 32];
+        if ((t & 31) == 0) {
+            s_sum[t >> 5] = ss;
+            s_max[t >> 5] = mx;
+        }
+        __syncthreads();
+        // every warp reduces the warps' values for itself
+        const int w = t & 31;
+        ss = w < T / 32 ? s_sum[w] : 0.f;
+        mx = w < T / 32 ? s_max[w] : 0;
+        if constexpr (NORM) ss = warp_sum(ss);
+        mx = __reduce_max_sync(0xffffffffu, mx);
     }
-    __syncthreads();
-    ss = 0.f;
-    mx = 0;
-    for (int w = 0; w < 8; ++w) {
-        ss += s_sum[w];
-        mx = max(mx, s_max[w]);
+    const RowScale rs = row_scale(mx, NORM ? rsqrtf(ss / static_cast<float>(D) + a.eps) : 1.f);
+    if (t == 0) a.scale[row] = rs.scale;
+    const uint32_t live = rs.inv == 0.f ? 0u : 0xFFFFFFFFu;   // a row without a scale has codes 0, whatever it holds
+#pragma unroll
+    for (int v = 0; v < V; ++v) {
+        const uint32_t lo = codes4(s[v][0], s[v][1], s[v][2], s[v][3], rs.inv) & live;
+        const uint32_t hi = codes4(s[v][4], s[v][5], s[v][6], s[v][7], rs.inv) & live;
+        if (whole(v)) *reinterpret_cast<uint2*>(q + at(v, 0)) = make_uint2(lo, hi);
+        else {
+#pragma unroll
+            for (int j = 0; j < 8; ++j)
+                if (at(v, j) < D) q[at(v, j)] = static_cast<int8_t>((j < 4 ? lo : hi) >> (8 * (j & 3)));
+        }
     }
-    const RowScale rs = row_scale(mx, NORM ? rsqrtf(ss / D + eps) : 1.f);
-    for (int i = threadIdx.x; i < D; i += 256) {
-        const float s = value(i);
-        if (delta) out[row * ldo + i] = from_f32<XT>(s);
-        q[row * ldq + i] = static_cast<int8_t>(code_of(NORM ? s * g[i] : s, rs.inv));
-    }
-    if (threadIdx.x == 0) scale[row] = rs.scale;
 }
 
 // One thread an output, 16 x 16 outputs a block, K by 64 codes through shared memory.

@@ -1676,30 +1676,50 @@ static uint32_t* i8_error_word(int dev)
 
 static long long i8_bytes(int type) { return type == kI8F32 ? 4 : 2; }
 
-template <bool NORM, typename XT, typename DT>
-static void launch_rows_i8_t(const void* x, const void* delta, const float* g, void* out, void* q, float* scale,
-                             int M, int D, long long ldx, long long ldd, long long ldo, long long ldq, float eps,
-                             cudaStream_t s)
+template <typename XT, typename DT, bool NORM, bool VEC, int T, int V>
+static void launch_rows_i8_cfg(const RowsI8& a, int num_sms, cudaStream_t s)
 {
-    launch_k(rows_i8_kernel<XT, DT, NORM>, dim3(static_cast<unsigned>(M)), dim3(256), 0, s, static_cast<const XT*>(x),
-             static_cast<const DT*>(delta), g, static_cast<XT*>(out), static_cast<int8_t*>(q), scale, D, ldx, ldd,
-             ldo, ldq, eps);
+    // a warp a row: eight rows a block, fewer while that leaves SMs without one
+    const int rows = T == 32 ? std::clamp(a.M / num_sms, 1, 8) : 1;
+    launch_k(rows_i8_kernel<XT, DT, NORM, VEC, T, V>, dim3((a.M + rows - 1) / rows), dim3(T * rows), 0, s, a);
+}
+
+// The narrowest set of threads that holds a row: a warp up to 1,024 elements, then a block.
+template <typename XT, typename DT, bool NORM>
+static void launch_rows_i8_t(const RowsI8& a, int num_sms, cudaStream_t s)
+{
+    const auto starts = [&](const void* p, long long ld, uintptr_t unit, size_t es) {
+        return !p || (reinterpret_cast<uintptr_t>(p) % unit == 0 && (a.M == 1 || ld * es % unit == 0));
+    };
+    const bool vec = starts(a.x, a.ldx, 16, sizeof(XT)) && starts(a.delta, a.ldd, 16, sizeof(DT)) &&
+                     starts(a.out, a.ldo, 16, sizeof(XT)) && starts(a.q, a.ldq, 8, 1) && starts(a.g, 0, 16, 4);
+    if (vec) {
+        if (a.D <= 512) launch_rows_i8_cfg<XT, DT, NORM, true, 32, 2>(a, num_sms, s);
+        else if (a.D <= 1024) launch_rows_i8_cfg<XT, DT, NORM, true, 32, 4>(a, num_sms, s);
+        else if (a.D <= 2048) launch_rows_i8_cfg<XT, DT, NORM, true, 128, 2>(a, num_sms, s);
+        else if (a.D <= 4096) launch_rows_i8_cfg<XT, DT, NORM, true, 128, 4>(a, num_sms, s);
+        else if (a.D <= 8192) launch_rows_i8_cfg<XT, DT, NORM, true, 256, 4>(a, num_sms, s);
+        else launch_rows_i8_cfg<XT, DT, NORM, true, 1024, 4>(a, num_sms, s);
+    } else {
+        if (a.D <= 1024) launch_rows_i8_cfg<XT, DT, NORM, false, 32, 4>(a, num_sms, s);
+        else if (a.D <= 8192) launch_rows_i8_cfg<XT, DT, NORM, false, 256, 4>(a, num_sms, s);
+        else launch_rows_i8_cfg<XT, DT, NORM, false, 1024, 4>(a, num_sms, s);
+    }
 }
 
 // k_rmsnorm_i8 (NORM) and k_quant_i8: x and delta of the types that the entry points take.
-template <bool NORM>
-static void launch_rows_i8(int x_type, int delta_type, const void* x, const void* delta, const float* g, void* out,
-                           void* q, float* scale, int M, int D, long long ldx, long long ldd, long long ldo,
-                           long long ldq, float eps, cudaStream_t s)
+template <bool NORM> static void launch_rows_i8(int x_type, int delta_type, const RowsI8& a, cudaStream_t s)
 {
-    auto go = [&](auto xt, auto dt) {
-        launch_rows_i8_t<NORM, decltype(xt), decltype(dt)>(x, delta, g, out, q, scale, M, D, ldx, ldd, ldo, ldq, eps, s);
-    };
-    if (x_type == kI8F16) go(__half(), __half());
-    else if (x_type == kI8BF16) go(__nv_bfloat16(), __nv_bfloat16());
-    else if (!NORM || delta_type == kI8F32) go(float(), float());
-    else if (delta_type == kI8F16) go(float(), __half());
-    else go(float(), __nv_bfloat16());
+    int dev = 0, sms = 0;
+    RT(cudaGetDevice(&dev));
+    RT(cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, dev));
+    if (x_type == kI8F16) launch_rows_i8_t<__half, __half, NORM>(a, sms, s);
+    else if (x_type == kI8BF16) launch_rows_i8_t<__nv_bfloat16, __nv_bfloat16, NORM>(a, sms, s);
+    else if (!NORM || !a.delta || delta_type == kI8F32) launch_rows_i8_t<float, float, NORM>(a, sms, s);
+    else if constexpr (NORM) {
+        if (delta_type == kI8F16) launch_rows_i8_t<float, __half, NORM>(a, sms, s);
+        else launch_rows_i8_t<float, __nv_bfloat16, NORM>(a, sms, s);
+    }
 }
 
 // What an int8 product is called with.
@@ -2298,8 +2318,9 @@ CUDANET_API int cudanet_k_rmsnorm_i8(int x_type, int delta_type, const void* x, 
         } else if (out) {
             throw std::runtime_error(std::string(who) + ": out without delta: there is no sum to store");
         }
-        mf::launch_rows_i8<true>(x_type, delta ? delta_type : x_type, x, delta, g, out, q, scale, M, D, ldx, ldd, ldo,
-                                 ldq, eps, static_cast<cudaStream_t>(stream));
+        mf::launch_rows_i8<true>(x_type, delta_type,
+                                 {x, delta, g, out, static_cast<int8_t*>(q), scale, M, D, ldx, ldd, ldo, ldq, eps},
+                                 static_cast<cudaStream_t>(stream));
         return 0;
     });
 }
@@ -2319,7 +2340,9 @@ CUDANET_API int cudanet_k_quant_i8(int x_type, const void* x, void* q, float* sc
         mf::need_ptr(who, "scale", scale, 4);
         mf::need_pitch(who, "ldx", ldx, D, M);
         mf::need_pitch(who, "ldq", ldq, D, M);
-        mf::launch_rows_i8<false>(x_type, x_type, x, nullptr, nullptr, nullptr, q, scale, M, D, ldx, 0, 0, ldq, 0.f,
+        mf::launch_rows_i8<false>(x_type, x_type,
+                                  {x, nullptr, nullptr, nullptr, static_cast<int8_t*>(q), scale, M, D, ldx, 0, 0, ldq,
+                                   0.f},
                                   static_cast<cudaStream_t>(stream));
         return 0;
     });
