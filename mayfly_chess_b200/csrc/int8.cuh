@@ -54,29 +54,38 @@ struct RowsI8 {
     float eps;
 };
 
-// 8 neighbouring elements from an address on 16 bytes
-__device__ __forceinline__ void load8(const float* p, float (&v)[8])
-{
-    const float4 a = __ldg(reinterpret_cast<const float4*>(p)), b = __ldg(reinterpret_cast<const float4*>(p) + 1);
-    v[0] = a.x, v[1] = a.y, v[2] = a.z, v[3] = a.w, v[4] = b.x, v[5] = b.y, v[6] = b.z, v[7] = b.w;
-}
-__device__ __forceinline__ void load8(const __nv_bfloat16* p, float (&v)[8])
-{
-    const uint4 a = __ldg(reinterpret_cast<const uint4*>(p));
-    const uint32_t w[4] = {a.x, a.y, a.z, a.w};
+// 8 elements as they lie in memory, so that all of a thread's loads are on their way before the first is converted.
+template <typename T> struct Raw8 {
+    uint4 w;
+    __device__ __forceinline__ void load(const T* p) { w = __ldg(reinterpret_cast<const uint4*>(p)); }   // on 16 bytes
+    __device__ __forceinline__ void zero() { w = make_uint4(0, 0, 0, 0); }
+    __device__ __forceinline__ void get(float (&v)[8]) const
+    {
+        const uint32_t u[4] = {w.x, w.y, w.z, w.w};
 #pragma unroll
-    for (int i = 0; i < 4; ++i) v[2 * i] = bf16_lo(w[i]), v[2 * i + 1] = bf16_hi(w[i]);
-}
-__device__ __forceinline__ void load8(const __half* p, float (&v)[8])
-{
-    const uint4 a = __ldg(reinterpret_cast<const uint4*>(p));
-    const uint32_t w[4] = {a.x, a.y, a.z, a.w};
-#pragma unroll
-    for (int i = 0; i < 4; ++i) {
-        const float2 f = __half22float2(*reinterpret_cast<const __half2*>(&w[i]));
-        v[2 * i] = f.x, v[2 * i + 1] = f.y;
+        for (int i = 0; i < 4; ++i) {
+            if constexpr (std::is_same<T, __half>::value) {
+                const float2 f = __half22float2(*reinterpret_cast<const __half2*>(&u[i]));
+                v[2 * i] = f.x, v[2 * i + 1] = f.y;
+            } else {
+                v[2 * i] = bf16_lo(u[i]), v[2 * i + 1] = bf16_hi(u[i]);
+            }
+        }
     }
-}
+};
+template <> struct Raw8<float> {
+    float4 a, b;
+    __device__ __forceinline__ void load(const float* p)
+    {
+        a = __ldg(reinterpret_cast<const float4*>(p));
+        b = __ldg(reinterpret_cast<const float4*>(p) + 1);
+    }
+    __device__ __forceinline__ void zero() { a = b = make_float4(0.f, 0.f, 0.f, 0.f); }
+    __device__ __forceinline__ void get(float (&v)[8]) const
+    {
+        v[0] = a.x, v[1] = a.y, v[2] = a.z, v[3] = a.w, v[4] = b.x, v[5] = b.y, v[6] = b.z, v[7] = b.w;
+    }
+};
 __device__ __forceinline__ void store8(float* p, const float (&v)[8])
 {
     reinterpret_cast<float4*>(p)[0] = make_float4(v[0], v[1], v[2], v[3]);
@@ -97,52 +106,81 @@ __device__ __forceinline__ uint32_t codes4(float a, float b, float c, float d, f
                        __byte_perm(code_byte(c, inv), code_byte(d, inv), 0x0040), 0x5410);
 }
 
-// T threads hold a row in registers (a warp each, T = 32, or a block), 8 V elements a thread, so x and delta are read
-// and out, q and scale written once: bound by HBM from about a thousand rows. VEC: neighbouring elements 8 at a time
-// (every row of every operand begins on 16 bytes, q's on 8); else element by element, T apart.
-template <typename XT, typename DT, bool NORM, bool VEC, int T, int V>
-__global__ void __launch_bounds__(T == 32 ? 256 : T) rows_i8_kernel(const RowsI8 a)
+// L threads hold a row in registers (8, 16 or 32 of a warp, or a block, L = 0), 8 V elements a thread, so x and delta
+// are read and out, q and scale written once: bound by HBM from about a thousand rows. VEC: neighbouring elements 8 at a
+// time (D a multiple of 8, every row of every operand begins on 16 bytes, q's on 8); else element by element.
+template <typename XT, typename DT, bool NORM, bool VEC, int L, int V>
+__global__ void __launch_bounds__(L ? 256 : 1024) rows_i8_kernel(const RowsI8 a)
 {
     griddep_wait();
     griddep_launch();
-    const int t = T == 32 ? threadIdx.x & 31 : threadIdx.x;
-    const size_t row = T == 32 ? (size_t)blockIdx.x * (blockDim.x >> 5) + (threadIdx.x >> 5) : blockIdx.x;
-    if (row >= (size_t)a.M) return;   // T = 32: a whole warp
+    const int T = L ? L : blockDim.x;
+    const int t = L ? threadIdx.x & (L - 1) : threadIdx.x;
+    const size_t row = L ? ((size_t)blockIdx.x * blockDim.x + threadIdx.x) / (L ? L : 1) : blockIdx.x;
+    // a warp that holds a row at all goes on as a whole, its threads without one with no elements
+    if (L && row - (threadIdx.x & 31) / (L ? L : 1) >= (size_t)a.M) return;
+    const int D = row < (size_t)a.M ? a.D : 0;
     const XT* __restrict__ x = static_cast<const XT*>(a.x) + row * a.ldx;
     const DT* __restrict__ delta = static_cast<const DT*>(a.delta) + row * a.ldd;
     XT* out = static_cast<XT*>(a.out) + row * a.ldo;
     int8_t* q = a.q + row * a.ldq;
     const bool add = NORM && a.delta;
-    const int D = a.D;
-    // element j of vector v of this thread; VEC: the last vector of the row may be cut
+    // element j of vector v of this thread
     auto at = [&](int v, int j) { return VEC ? 8 * (t + T * v) + j : t + T * (8 * v + j); };
-    auto whole = [&](int v) { return VEC && at(v, 8) <= D; };
 
-    float s[V][8];
-#pragma unroll
-    for (int v = 0; v < V; ++v) {
-        if (whole(v)) load8(x + at(v, 0), s[v]);
-        else {
-#pragma unroll
-            for (int j = 0; j < 8; ++j) s[v][j] = at(v, j) < D ? to_f32(x[at(v, j)]) : 0.f;
-        }
-    }
-    if (add) {
-        float d[V][8];
+    float s[V][8], d[V][8];
+    if constexpr (VEC) {
+        Raw8<XT> rx[V];
+        Raw8<DT> rd[V];
 #pragma unroll
         for (int v = 0; v < V; ++v) {
-            if (whole(v)) load8(delta + at(v, 0), d[v]);
-            else {
+            rx[v].zero();
+            if (at(v, 0) < D) rx[v].load(x + at(v, 0));
+        }
+        if (add) {
 #pragma unroll
-                for (int j = 0; j < 8; ++j) d[v][j] = at(v, j) < D ? to_f32(delta[at(v, j)]) : 0.f;
+            for (int v = 0; v < V; ++v) {
+                rd[v].zero();
+                if (at(v, 0) < D) rd[v].load(delta + at(v, 0));
+            }
+        }
+#pragma unroll
+        for (int v = 0; v < V; ++v) {
+            rx[v].get(s[v]);
+            if (add) rd[v].get(d[v]);
+        }
+    } else {
+        XT rx[V][8];
+        DT rd[V][8];
+#pragma unroll
+        for (int v = 0; v < V; ++v) {
+#pragma unroll
+            for (int j = 0; j < 8; ++j) rx[v][j] = at(v, j) < D ? x[at(v, j)] : from_f32<XT>(0.f);
+        }
+        if (add) {
+#pragma unroll
+            for (int v = 0; v < V; ++v) {
+#pragma unroll
+                for (int j = 0; j < 8; ++j) rd[v][j] = at(v, j) < D ? delta[at(v, j)] : from_f32<DT>(0.f);
             }
         }
 #pragma unroll
         for (int v = 0; v < V; ++v) {
 #pragma unroll
+            for (int j = 0; j < 8; ++j) {
+                s[v][j] = to_f32(rx[v][j]);
+                if (add) d[v][j] = to_f32(rd[v][j]);
+            }
+        }
+    }
+    if (add) {
+#pragma unroll
+        for (int v = 0; v < V; ++v) {
+#pragma unroll
             for (int j = 0; j < 8; ++j) s[v][j] = to_f32(from_f32<XT>(s[v][j] + d[v][j]));
-            if (whole(v)) store8(out + at(v, 0), s[v]);
-            else {
+            if constexpr (VEC) {
+                if (at(v, 0) < D) store8(out + at(v, 0), s[v]);
+            } else {
 #pragma unroll
                 for (int j = 0; j < 8; ++j)
                     if (at(v, j) < D) out[at(v, j)] = from_f32<XT>(s[v][j]);
@@ -155,8 +193,12 @@ __global__ void __launch_bounds__(T == 32 ? 256 : T) rows_i8_kernel(const RowsI8
     for (int v = 0; v < V; ++v) {
         if constexpr (NORM) {
             float g[8];
-            if (whole(v)) load8(a.g + at(v, 0), g);
-            else {
+            if constexpr (VEC) {
+                Raw8<float> rg;
+                rg.zero();
+                if (at(v, 0) < D) rg.load(a.g + at(v, 0));
+                rg.get(g);
+            } else {
 #pragma unroll
                 for (int j = 0; j < 8; ++j) g[j] = at(v, j) < D ? __ldg(a.g + at(v, j)) : 0.f;
             }
@@ -169,11 +211,19 @@ __global__ void __launch_bounds__(T == 32 ? 256 : T) rows_i8_kernel(const RowsI8
 #pragma unroll
         for (int j = 0; j < 8; ++j) mx = max(mx, __float_as_uint(s[v][j]) & 0x7FFFFFFFu);
     }
-    if constexpr (NORM) ss = warp_sum(ss);
-    mx = __reduce_max_sync(0xffffffffu, mx);
-    if constexpr (T > 32) {
-        __shared__ float s_sum[T / 32];
-        __shared__ uint32_t s_max[T / 32];
+    if constexpr (L == 8 || L == 16) {
+#pragma unroll
+        for (int o = L / 2; o > 0; o >>= 1) {
+            if constexpr (NORM) ss += __shfl_xor_sync(0xffffffffu, ss, o);
+            mx = max(mx, __shfl_xor_sync(0xffffffffu, mx, o));
+        }
+    } else {
+        if constexpr (NORM) ss = warp_sum(ss);
+        mx = __reduce_max_sync(0xffffffffu, mx);
+    }
+    if constexpr (L == 0) {
+        __shared__ float s_sum[32];
+        __shared__ uint32_t s_max[32];
         if ((t & 31) == 0) {
             s_sum[t >> 5] = ss;
             s_max[t >> 5] = mx;
@@ -182,19 +232,20 @@ __global__ void __launch_bounds__(T == 32 ? 256 : T) rows_i8_kernel(const RowsI8
         // every warp reduces the warps' values for itself
         const int w = t & 31;
         ss = w < T / 32 ? s_sum[w] : 0.f;
-        mx = w < T / 32 ? s_max[w] : 0;
+        mx = w < T / 32 ? s_max[w] : 0u;
         if constexpr (NORM) ss = warp_sum(ss);
         mx = __reduce_max_sync(0xffffffffu, mx);
     }
-    const RowScale rs = row_scale(mx, NORM ? rsqrtf(ss / static_cast<float>(D) + a.eps) : 1.f);
-    if (t == 0) a.scale[row] = rs.scale;
+    const RowScale rs = row_scale(mx, NORM ? rsqrtf(ss / static_cast<float>(a.D) + a.eps) : 1.f);
+    if (t == 0 && D) a.scale[row] = rs.scale;
     const uint32_t live = rs.inv == 0.f ? 0u : 0xFFFFFFFFu;   // a row without a scale has codes 0, whatever it holds
 #pragma unroll
     for (int v = 0; v < V; ++v) {
         const uint32_t lo = codes4(s[v][0], s[v][1], s[v][2], s[v][3], rs.inv) & live;
         const uint32_t hi = codes4(s[v][4], s[v][5], s[v][6], s[v][7], rs.inv) & live;
-        if (whole(v)) *reinterpret_cast<uint2*>(q + at(v, 0)) = make_uint2(lo, hi);
-        else {
+        if constexpr (VEC) {
+            if (at(v, 0) < D) *reinterpret_cast<uint2*>(q + at(v, 0)) = make_uint2(lo, hi);
+        } else {
 #pragma unroll
             for (int j = 0; j < 8; ++j)
                 if (at(v, j) < D) q[at(v, j)] = static_cast<int8_t>((j < 4 ? lo : hi) >> (8 * (j & 3)));

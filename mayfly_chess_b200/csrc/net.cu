@@ -1676,34 +1676,56 @@ static uint32_t* i8_error_word(int dev)
 
 static long long i8_bytes(int type) { return type == kI8F32 ? 4 : 2; }
 
-template <typename XT, typename DT, bool NORM, bool VEC, int T, int V>
+template <typename XT, typename DT, bool NORM, bool VEC, int L, int V>
 static void launch_rows_i8_cfg(const RowsI8& a, int num_sms, cudaStream_t s)
 {
-    // a warp a row: eight rows a block, fewer while that leaves SMs without one
-    const int rows = T == 32 ? std::clamp(a.M / num_sms, 1, 8) : 1;
-    launch_k(rows_i8_kernel<XT, DT, NORM, VEC, T, V>, dim3((a.M + rows - 1) / rows), dim3(T * rows), 0, s, a);
+    int rows = 1, threads = (a.D + 8 * V - 1) / (8 * V);   // a block a row
+    if (L) {
+        // part of a warp a row: 256 threads a block, fewer while that leaves SMs without one
+        const int warps = (a.M + 32 / (L ? L : 32) - 1) / (32 / (L ? L : 32));
+        threads = 32 * std::clamp(warps / num_sms, 1, 8);
+        rows = threads / (L ? L : 32);
+    }
+    launch_k(rows_i8_kernel<XT, DT, NORM, VEC, L, V>, dim3((a.M - 1) / rows + 1), dim3((threads + 31) / 32 * 32), 0, s,
+             a);
 }
 
-// The narrowest set of threads that holds a row: a warp up to 1,024 elements, then a block.
+// Part of a warp up to 1,024 elements (2,048 for the 16-bit quantiser), then a block a row: as few threads as hold the
+// row with enough loads on their way. Measured (GB/s, 66,560 x 2,048 bf16 quantised: a warp of 8 vectors a thread 6,946,
+// a block of 4 5,843; 4,097 x 8,192 bf16 norm: blocks of 4 vectors 6,138, of 2 5,312, of 1 4,327). Rows that are read
+// element by element: 20,871 x 727 f16 quantised in a warp 2,829, in a block 1,978; 16,000 x 4,001 f16 norm in blocks of
+// 8 elements a thread 2,285, of 16 1,619, of 32 1,488, the quantiser there 1,822, 2,327 and 1,960.
 template <typename XT, typename DT, bool NORM>
 static void launch_rows_i8_t(const RowsI8& a, int num_sms, cudaStream_t s)
 {
     const auto starts = [&](const void* p, long long ld, uintptr_t unit, size_t es) {
         return !p || (reinterpret_cast<uintptr_t>(p) % unit == 0 && (a.M == 1 || ld * es % unit == 0));
     };
-    const bool vec = starts(a.x, a.ldx, 16, sizeof(XT)) && starts(a.delta, a.ldd, 16, sizeof(DT)) &&
+    const bool vec = a.D % 8 == 0 && starts(a.x, a.ldx, 16, sizeof(XT)) && starts(a.delta, a.ldd, 16, sizeof(DT)) &&
                      starts(a.out, a.ldo, 16, sizeof(XT)) && starts(a.q, a.ldq, 8, 1) && starts(a.g, 0, 16, 4);
+    const int D = a.D;
     if (vec) {
-        if (a.D <= 512) launch_rows_i8_cfg<XT, DT, NORM, true, 32, 2>(a, num_sms, s);
-        else if (a.D <= 1024) launch_rows_i8_cfg<XT, DT, NORM, true, 32, 4>(a, num_sms, s);
-        else if (a.D <= 2048) launch_rows_i8_cfg<XT, DT, NORM, true, 128, 2>(a, num_sms, s);
-        else if (a.D <= 4096) launch_rows_i8_cfg<XT, DT, NORM, true, 128, 4>(a, num_sms, s);
-        else if (a.D <= 8192) launch_rows_i8_cfg<XT, DT, NORM, true, 256, 4>(a, num_sms, s);
-        else launch_rows_i8_cfg<XT, DT, NORM, true, 1024, 4>(a, num_sms, s);
+        // the quantiser of 16-bit rows has a third of the norm's bytes a vector in flight: more vectors a thread
+        constexpr bool Q16 = sizeof(XT) == 2 && !NORM;
+        constexpr int BV = sizeof(XT) == 2 ? 4 : 2;
+        if (D <= 64) launch_rows_i8_cfg<XT, DT, NORM, true, 8, 1>(a, num_sms, s);
+        else if (D <= 128) launch_rows_i8_cfg<XT, DT, NORM, true, 16, 1>(a, num_sms, s);
+        else if (D <= 256) launch_rows_i8_cfg<XT, DT, NORM, true, 32, 1>(a, num_sms, s);
+        else if (D <= 512) launch_rows_i8_cfg<XT, DT, NORM, true, 32, 2>(a, num_sms, s);
+        else if (D <= 768) launch_rows_i8_cfg<XT, DT, NORM, true, 32, 3>(a, num_sms, s);
+        else if (D <= 1024) launch_rows_i8_cfg<XT, DT, NORM, true, 32, 4>(a, num_sms, s);
+        else if (Q16 && D <= 1536) launch_rows_i8_cfg<XT, DT, NORM, true, 32, Q16 ? 6 : 4>(a, num_sms, s);
+        else if (Q16 && D <= 2048) launch_rows_i8_cfg<XT, DT, NORM, true, 32, Q16 ? 8 : 4>(a, num_sms, s);
+        else if (D <= 16384) launch_rows_i8_cfg<XT, DT, NORM, true, 0, BV>(a, num_sms, s);
+        else launch_rows_i8_cfg<XT, DT, NORM, true, 0, Q16 ? 8 : 4>(a, num_sms, s);
     } else {
-        if (a.D <= 1024) launch_rows_i8_cfg<XT, DT, NORM, false, 32, 4>(a, num_sms, s);
-        else if (a.D <= 8192) launch_rows_i8_cfg<XT, DT, NORM, false, 256, 4>(a, num_sms, s);
-        else launch_rows_i8_cfg<XT, DT, NORM, false, 1024, 4>(a, num_sms, s);
+        constexpr int BV = NORM ? 1 : 2;
+        if (D <= 256) launch_rows_i8_cfg<XT, DT, NORM, false, 32, 1>(a, num_sms, s);
+        else if (D <= 512) launch_rows_i8_cfg<XT, DT, NORM, false, 32, 2>(a, num_sms, s);
+        else if (D <= 768) launch_rows_i8_cfg<XT, DT, NORM, false, 32, 3>(a, num_sms, s);
+        else if (D <= 1024) launch_rows_i8_cfg<XT, DT, NORM, false, 32, 4>(a, num_sms, s);
+        else if (D <= 8192 * BV) launch_rows_i8_cfg<XT, DT, NORM, false, 0, BV>(a, num_sms, s);
+        else launch_rows_i8_cfg<XT, DT, NORM, false, 0, 4>(a, num_sms, s);
     }
 }
 
