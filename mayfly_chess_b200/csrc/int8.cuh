@@ -253,40 +253,202 @@ __global__ void __launch_bounds__(L ? 256 : 1024) rows_i8_kernel(const RowsI8 a)
     }
 }
 
-// One thread an output, 16 x 16 outputs a block, K by 64 codes through shared memory.
-template <typename TO, int EPI>
-__global__ void __launch_bounds__(256) gemm_i8_simple_kernel(const int8_t* __restrict__ A, const int8_t* __restrict__ W,
-                                                             const float* __restrict__ rowscale,
-                                                             const float* __restrict__ colscale,
-                                                             const float* __restrict__ bias, TO* C, int M, int N, int K,
-                                                             long long lda, long long ldw, long long ldc)
+// ------------------------------------------------------------------------------------------------ few rows
+// The product for few rows of A, and for outputs whose rows are not whole 16-byte units. The weight takes the 128 lanes
+// of the tensor-core instruction (M = 128 rows of W) and the tokens its columns (N = TN rows of A), so that a few tokens
+// waste little and a thread of the epilogue owns an output channel: its column scale and bias stay in two registers,
+// and a warp stores 32 neighbouring channels of a row, wherever the row begins. K is split over a cluster of S CTAs,
+// which fills the GPU where the tiles alone do not: each CTA leaves its exact int32 partial sums in its shared memory
+// and sums a share of the tokens over the cluster through distributed shared memory. No workspace, no atomics.
+template <int TN> struct I8SplitCfg {
+    static constexpr uint32_t W_BYTES = 128 * 128, A_BYTES = TN * 128, STAGE_BYTES = W_BYTES + A_BYTES;
+    static constexpr int STAGES = TN == 128 ? 3 : TN == 64 ? 4 : 5;   // two CTAs an SM
+    static constexpr uint32_t TMEM_COLS = TN < 32 ? 32 : TN;
+    static constexpr size_t SMEM = 1024 + STAGES * STAGE_BYTES + 4 * TN + 16 * STAGES + 32;
+    static constexpr int THREADS = 192;
+    static_assert(STAGES * STAGE_BYTES >= 4 * 128 * TN, "the partial sums lie where the stages were");
+};
+
+// The outputs and vectors of a product.
+struct I8Out {
+    const float *rowscale, *colscale, *bias;
+    void* C;
+    long long ldc;
+    int M, N, K, n_tiles;
+};
+
+template <typename TO, int EPI, int TN>
+__global__ void __launch_bounds__(192) gemm_i8_split_kernel(const __grid_constant__ CUtensorMap tmA,
+                                                            const __grid_constant__ CUtensorMap tmW, const I8Out p,
+                                                            uint32_t* err)
 {
-    griddep_wait();
-    griddep_launch();
-    __shared__ int sa[16][17], sw[16][17];
-    const int tx = threadIdx.x & 15, ty = threadIdx.x >> 4;
-    const long long m0 = (long long)blockIdx.y * 16, n0 = (long long)blockIdx.x * 16;
-    auto word = [&](const int8_t* p, long long ld, long long r, long long rows, int k) {
-        uint32_t w = 0;
-        if (r < rows)
-            for (int b = 0; b < 4; ++b)
-                if (k + b < K) w |= (uint32_t)(uint8_t)p[r * ld + k + b] << (8 * b);
-        return (int)w;
-    };
-    int acc = 0;
-    for (int k0 = 0; k0 < K; k0 += 64) {
-        sa[ty][tx] = word(A, lda, m0 + ty, M, k0 + 4 * tx);
-        sw[ty][tx] = word(W, ldw, n0 + ty, N, k0 + 4 * tx);
-        __syncthreads();
-        for (int j = 0; j < 16; ++j) acc = __dp4a(sa[ty][j], sw[tx][j], acc);
-        __syncthreads();
+    using C = I8SplitCfg<TN>;
+    extern __shared__ uint8_t smem_raw[];
+    uint8_t* const sW = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
+    uint8_t* const sA = sW + C::STAGES * C::W_BYTES;
+    float* const s_rowscale = reinterpret_cast<float*>(sA + C::STAGES * C::A_BYTES);
+    uint64_t* const full = reinterpret_cast<uint64_t*>(s_rowscale + TN);
+    uint64_t* const empty = full + C::STAGES;
+    uint64_t* const done = empty + C::STAGES;      // every MMA of this CTA has completed
+    uint32_t* const tmem_slot = reinterpret_cast<uint32_t*>(done + 1);
+
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    const uint32_t S = cluster_nctarank(), rank = cluster_ctarank();
+    const int tile = blockIdx.x / S;
+    const int n0 = tile % p.n_tiles * 128, m0 = tile / p.n_tiles * TN;
+    // this CTA's 128-byte blocks of K (at least one: S is no more than there are)
+    const int blocks = (p.K + 127) / 128;
+    const int kb0 = static_cast<int>((long long)blocks * rank / S), kb1 = static_cast<int>((long long)blocks * (rank + 1) / S);
+
+    if (threadIdx.x == 0) {
+        for (int s = 0; s < C::STAGES; ++s) {
+            mbar_init(&full[s], 1);
+            mbar_init(&empty[s], 1);
+        }
+        mbar_init(done, 1);
+        fence_barrier_init();
+        tma_prefetch_desc(&tmA);
+        tma_prefetch_desc(&tmW);
     }
-    const long long m = m0 + ty, n = n0 + tx;
-    if (m >= M || n >= N) return;
-    float v = i8_value(acc, rowscale[m], colscale[n], bias ? bias[n] : 0.f);
-    if constexpr (EPI == kEpiBiasGelu) v = gelu_pair<false, true>(pk2(v, v), GeluK(1.0f)).x;
-    if constexpr (EPI == kEpiResidual) v += C[m * ldc + n];
-    C[m * ldc + n] = from_f32<TO>(v);
+    if (warp == 1) {
+        tmem_alloc(tmem_slot, C::TMEM_COLS);
+        tmem_relinquish();
+    }
+    tc_fence_before();
+    __syncthreads();
+    tc_fence_after();
+    const uint32_t tmem = *tmem_slot;
+    if (threadIdx.x == 0) griddep_launch();
+
+    const int n = n0 + (warp & 3) * 32 + lane;                     // the epilogue's channel of this thread
+    const int tokens = p.M - m0 < TN ? p.M - m0 : TN;
+    const bool in = n < p.N;
+    float cs = 0.f, bias = 0.f;
+    bool ok = true;
+    TO* const c = static_cast<TO*>(p.C) + (size_t)m0 * p.ldc + n;
+    const auto value = [&](int acc, int t) {
+        const float v = i8_value(acc, s_rowscale[t], cs, bias);
+        if constexpr (EPI == kEpiBiasGelu) return gelu_pair<false, true>(pk2(v, v), GeluK(1.0f)).x;
+        return v;
+    };
+    int* const part = reinterpret_cast<int*>(sW);                  // [tokens][128] partial sums
+
+    if (warp == 0) {
+        if (lane == 0) {
+            griddep_wait();
+            int stage = 0;
+            uint32_t phase = 0;
+            int kb = kb0;
+            for (; kb < kb1; ++kb) {
+                if (!mbar_wait(&empty[stage], phase ^ 1u, err, kErrSmemEmpty)) break;
+                mbar_arrive_expect_tx(&full[stage], C::STAGE_BYTES);
+                tma_load_2d(sW + stage * C::W_BYTES, &tmW, &full[stage], kb * 128, n0);
+                tma_load_2d(sA + stage * C::A_BYTES, &tmA, &full[stage], kb * 128, m0);
+                if (++stage == C::STAGES) {
+                    stage = 0;
+                    phase ^= 1u;
+                }
+            }
+            // every copy that was started has landed before the CTA can leave: the last ones, stage by stage
+            const int issued = kb - kb0;
+            for (int i = issued > C::STAGES ? issued - C::STAGES : 0; i < issued; ++i)
+                mbar_wait(&full[i % C::STAGES], (i / C::STAGES) & 1, err, kErrTmaFull);
+        }
+    } else if (warp == 1) {
+        if (lane == 0) {
+            constexpr uint32_t idesc = idesc_i8(128, TN);
+            int stage = 0;
+            uint32_t phase = 0;
+            for (int kb = kb0; kb < kb1; ++kb) {
+                if (!mbar_wait(&full[stage], phase, err, kErrTmaFull)) break;
+                tc_fence_after();
+                const uint32_t w = smem_u32(sW + stage * C::W_BYTES), a = smem_u32(sA + stage * C::A_BYTES);
+#pragma unroll
+                for (int k = 0; k < 4; ++k)
+                    umma_i8(tmem, sdesc_sw128(w + 32u * k), sdesc_sw128(a + 32u * k), idesc,
+                            kb != kb0 || k != 0 ? 1u : 0u);
+                umma_commit(&empty[stage]);
+                if (++stage == C::STAGES) {
+                    stage = 0;
+                    phase ^= 1u;
+                }
+            }
+            umma_commit(done);
+            mbar_wait(done, 0, err, kErrTmemFull);
+        }
+    } else {
+        griddep_wait();
+        const int e = threadIdx.x - 64;
+        if (e < tokens) s_rowscale[e] = __ldg(p.rowscale + m0 + e);
+        if (in) {
+            cs = __ldg(p.colscale + n);
+            if (p.bias) bias = __ldg(p.bias + n);
+        }
+        named_barrier(1, 128);
+        ok = __all_sync(0xffffffffu, mbar_wait(done, 0, err, kErrTmemFull));
+        tc_fence_after();
+        const uint32_t t_lane = tmem + (static_cast<uint32_t>((warp & 3) * 32) << 16);
+        for (int t0 = 0; ok && t0 < tokens; t0 += 16) {
+            uint32_t a[16];
+            tmem_ld_32x32b_x16(t_lane + static_cast<uint32_t>(t0), a);
+            tmem_ld_wait();
+            if (S > 1) {
+#pragma unroll
+                for (int i = 0; i < 16; ++i)
+                    if (t0 + i < tokens) part[(t0 + i) * 128 + (warp & 3) * 32 + lane] = static_cast<int>(a[i]);
+            } else if (in) {
+                float old[16];
+                if constexpr (EPI == kEpiResidual) {
+#pragma unroll
+                    for (int i = 0; i < 16; ++i) old[i] = t0 + i < tokens ? c[(size_t)(t0 + i) * p.ldc] : 0.f;
+                }
+#pragma unroll
+                for (int i = 0; i < 16; ++i) {
+                    if (t0 + i < tokens) {
+                        float v = value(static_cast<int>(a[i]), t0 + i);
+                        if constexpr (EPI == kEpiResidual) v += old[i];
+                        c[(size_t)(t0 + i) * p.ldc] = from_f32<TO>(v);
+                    }
+                }
+            }
+        }
+    }
+
+    __syncwarp();
+    if (S > 1) {
+        cluster_sync();            // every CTA's partial sums are written
+        if (warp >= 2 && ok && in) {
+            const int ta = static_cast<int>(tokens * rank / S), tb = static_cast<int>(tokens * (rank + 1) / S);
+            const uint32_t mine = smem_u32(part) + 4u * static_cast<uint32_t>((warp & 3) * 32 + lane);
+            for (int t = ta; t < tb; t += 4) {
+                int sum[4] = {0, 0, 0, 0};
+#pragma unroll
+                for (uint32_t r = 0; r < 8; ++r) {
+                    if (r < S) {
+                        const uint32_t from = mapa_shared(mine, r);
+#pragma unroll
+                        for (int i = 0; i < 4; ++i)
+                            if (t + i < tb) sum[i] += static_cast<int>(ld_cluster(from + 512u * static_cast<uint32_t>(t + i)));
+                    }
+                }
+#pragma unroll
+                for (int i = 0; i < 4; ++i) {
+                    if (t + i < tb) {
+                        float v = value(sum[i], t + i);
+                        TO* at = c + (size_t)(t + i) * p.ldc;
+                        if constexpr (EPI == kEpiResidual) v += *at;
+                        *at = from_f32<TO>(v);
+                    }
+                }
+            }
+        }
+        __syncwarp();
+        cluster_sync();            // no CTA reads another's shared memory any more
+    }
+    tc_fence_before();
+    __syncthreads();
+    tc_fence_after();
+    if (warp == 1) tmem_dealloc(tmem, C::TMEM_COLS);
 }
 
 }  // namespace mf

@@ -1754,12 +1754,50 @@ struct GemmI8 {
 };
 
 // The kernels of an int8 product: the choice of `kernel` -1, else what the caller asks for.
-enum I8Kernel : int { kI8Single = 0, kI8Pair = 1 };
+enum I8Kernel : int { kI8Single = 0, kI8Pair = 1, kI8Split = 2 };   // kI8Split + S: the split over S CTAs
 
 static int pick_i8_kernel(const GemmI8& p, int num_sms)
 {
     const long long tiles = ((p.M + 255LL) / 256) * ((p.N + 255) / 256);
-    return tiles >= num_sms / 2 ? kI8Pair : kI8Single;
+    return tiles >= num_sms / 2 ? kI8Pair : kI8Split;
+}
+
+template <typename TO, int EPI, int TN>
+static void launch_gemm_i8_split(const GemmI8& p, const CUtensorMap& mw, long long pitch_a, int split, int num_sms,
+                                 uint32_t* err, cudaStream_t s)
+{
+    using C = I8SplitCfg<TN>;
+    static bool attr[64] = {};
+    int dev = 0;
+    RT(cudaGetDevice(&dev));
+    if (dev < 0 || dev >= 64) throw std::runtime_error("cudanet_b200: device index out of range");
+    if (!attr[dev]) {
+        RT(cudaFuncSetAttribute(gemm_i8_split_kernel<TO, EPI, TN>, cudaFuncAttributeMaxDynamicSharedMemorySize,
+                                (int)C::SMEM));
+        attr[dev] = true;
+    }
+    const int n_tiles = (p.N + 127) / 128, blocks = (p.K + 127) / 128;
+    const long long tiles = (long long)n_tiles * ((p.M + TN - 1) / TN);
+    if (split == 0)
+        for (split = 1; split < 8 && tiles * split * 2 <= 2 * num_sms;) split *= 2;
+    while (split > blocks) split /= 2;
+    if (tiles * split > (1LL << 31) - 1) throw std::runtime_error("cudanet_k_gemm_i8: too many tiles");
+    const CUtensorMap ma = make_map(p.A, MapType::U8, p.K, p.M, pitch_a, 128, TN);
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = dim3(static_cast<unsigned>(tiles * split));
+    cfg.blockDim = dim3(C::THREADS);
+    cfg.dynamicSmemBytes = C::SMEM;
+    cfg.stream = s;
+    cudaLaunchAttribute la[2];
+    la[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    la[0].val.programmaticStreamSerializationAllowed = pdl_on() ? 1 : 0;
+    la[1].id = cudaLaunchAttributeClusterDimension;
+    la[1].val.clusterDim.x = static_cast<unsigned>(split);
+    la[1].val.clusterDim.y = la[1].val.clusterDim.z = 1;
+    cfg.attrs = la;
+    cfg.numAttrs = 2;
+    const I8Out out{p.rowscale, p.colscale, p.bias, p.C, p.ldc, p.M, p.N, p.K, n_tiles};
+    RT(cudaLaunchKernelEx(&cfg, gemm_i8_split_kernel<TO, EPI, TN>, ma, mw, out, err));
 }
 
 template <typename TO, int EPI>
@@ -1768,29 +1806,31 @@ static void launch_gemm_i8_t(const GemmI8& p, int kernel, cudaStream_t s)
     int dev = 0, sms = 0;
     RT(cudaGetDevice(&dev));
     RT(cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, dev));
+    uint32_t* err = i8_error_word(dev);
     // a TMA store writes whole 16-byte units, the last of a row past its end too: rows must be made of such units
     const bool units = reinterpret_cast<uintptr_t>(p.C) % 16 == 0 && p.N * sizeof(TO) % 16 == 0 &&
                        (p.M == 1 || p.ldc * sizeof(TO) % 16 == 0);
-    if (!units) {
-        launch_k(gemm_i8_simple_kernel<TO, EPI>, dim3((p.N + 15) / 16, (p.M + 15) / 16), dim3(256), 0, s,
-                 static_cast<const int8_t*>(p.A), static_cast<const int8_t*>(p.W), p.rowscale, p.colscale, p.bias,
-                 static_cast<TO*>(p.C), p.M, p.N, p.K, p.lda, p.ldw, p.ldc);
+    if (kernel < 0) kernel = pick_i8_kernel(p, sms);
+    if (!units && kernel < kI8Split) kernel = kI8Split;
+    const auto pitch = [](long long ld, int width, int rows) { return rows > 1 ? ld : (width + 15LL) / 16 * 16; };
+    const long long pa = pitch(p.lda, p.K, p.M);
+    const CUtensorMap mw = make_map(p.W, MapType::U8, p.K, p.N, pitch(p.ldw, p.K, p.N), 128, kernel == kI8Single ? 256 : 128);
+    if (kernel >= kI8Split) {
+        const int split = kernel - kI8Split;
+        if (p.M <= 16) launch_gemm_i8_split<TO, EPI, 16>(p, mw, pa, split, sms, err, s);
+        else if (p.M <= 32) launch_gemm_i8_split<TO, EPI, 32>(p, mw, pa, split, sms, err, s);
+        else if (p.M <= 64) launch_gemm_i8_split<TO, EPI, 64>(p, mw, pa, split, sms, err, s);
+        else launch_gemm_i8_split<TO, EPI, 128>(p, mw, pa, split, sms, err, s);
         return;
     }
-    if (kernel < 0) kernel = pick_i8_kernel(p, sms);
-    const auto pitch = [](long long ld, int width, int rows) { return rows > 1 ? ld : (width + 15LL) / 16 * 16; };
-    const CUtensorMap ma = make_map(p.A, MapType::U8, p.K, p.M, pitch(p.lda, p.K, p.M), 128, 128);
-    const CUtensorMap mb = make_map(p.W, MapType::U8, p.K, p.N, pitch(p.ldw, p.K, p.N), 128,
-                                    w_box_rows(kernel == kI8Pair ? kPairTile : 256));
+    const CUtensorMap ma = make_map(p.A, MapType::U8, p.K, p.M, pa, 128, 128);
     constexpr MapType t = std::is_same<TO, float>::value    ? MapType::F32
                           : std::is_same<TO, __half>::value ? MapType::F16
                                                             : MapType::BF16;
-    const CUtensorMap mc = make_map(p.C, t, p.N, p.M, p.M > 1 ? p.ldc : (p.N + 15LL) / 16 * 16, 128 / sizeof(TO), 32);
+    const CUtensorMap mc = make_map(p.C, t, p.N, p.M, pitch(p.ldc, p.N, p.M), 128 / sizeof(TO), 32);
     const EpiArgs ep{p.bias, p.colscale, 1.f, 0, p.rowscale};
-    if (kernel == kI8Pair)
-        launch_gemm_pair<int8_t, TO, EPI>(ma, mb, mc, p.M, p.N, p.K, ep, i8_error_word(dev), s);
-    else
-        launch_gemm_bn<int8_t, TO, 256, EPI>(ma, mb, mc, p.M, p.N, p.K, ep, i8_error_word(dev), sms, s);
+    if (kernel == kI8Pair) launch_gemm_pair<int8_t, TO, EPI>(ma, mw, mc, p.M, p.N, p.K, ep, err, s);
+    else launch_gemm_bn<int8_t, TO, 256, EPI>(ma, mw, mc, p.M, p.N, p.K, ep, err, sms, s);
 }
 
 // A null pointer, or one whose address is no multiple of `align`, named in the reason.
@@ -2378,7 +2418,8 @@ CUDANET_API int cudanet_k_gemm_i8(int dtype, int epi, int kernel, const void* A,
         const char* who = "cudanet_k_gemm_i8";
         if (dtype != 0 && dtype != 1) throw std::runtime_error(std::string(who) + ": dtype must be 0 (f16) or 1 (bf16)");
         if (epi < 0 || epi > 3) throw std::runtime_error(std::string(who) + ": epi must be 0..3");
-        if (kernel < -1 || kernel > 1) throw std::runtime_error(std::string(who) + ": kernel must be -1, 0 or 1");
+        if (kernel < -1 || (kernel > 2 && kernel != 3 && kernel != 4 && kernel != 6 && kernel != 10))
+            throw std::runtime_error(std::string(who) + ": kernel must be -1, 0, 1, 2, 3, 4, 6 or 10");
         if (M < 0 || N < 1 || K < 1 || K > mf::kI8MaxK || M > mf::kI8MaxRows || N > mf::kI8MaxRows)
             throw std::runtime_error(std::string(who) + ": bad sizes (0 <= M, 1 <= N, both <= 2^30, 1 <= K <= 131071)");
         if (M == 0) return 0;
