@@ -264,8 +264,9 @@ template <int TN> struct I8SplitCfg {
     static constexpr uint32_t W_BYTES = 128 * 128, A_BYTES = TN * 128, STAGE_BYTES = W_BYTES + A_BYTES;
     static constexpr int STAGES = TN == 128 ? 3 : TN == 64 ? 4 : 5;   // two CTAs an SM
     static constexpr uint32_t TMEM_COLS = TN < 32 ? 32 : TN;
-    static constexpr size_t SMEM = 1024 + STAGES * STAGE_BYTES + 4 * TN + 16 * STAGES + 32;
-    static constexpr int THREADS = 192;
+    static constexpr size_t SMEM = 1024 + STAGES * STAGE_BYTES + 4 * (TN + 4) + 16 * STAGES + 32;
+    static constexpr int GROUPS = 4;                                  // of 4 epilogue warps, TN / 4 tokens each
+    static constexpr int THREADS = 64 + 128 * GROUPS;
     static_assert(STAGES * STAGE_BYTES >= 4 * 128 * TN, "the partial sums lie where the stages were");
 };
 
@@ -278,16 +279,16 @@ struct I8Out {
 };
 
 template <typename TO, int EPI, int TN>
-__global__ void __launch_bounds__(192) gemm_i8_split_kernel(const __grid_constant__ CUtensorMap tmA,
-                                                            const __grid_constant__ CUtensorMap tmW, const I8Out p,
-                                                            uint32_t* err)
+__global__ void __launch_bounds__(I8SplitCfg<TN>::THREADS, 2)
+gemm_i8_split_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant__ CUtensorMap tmW, const I8Out p,
+                     uint32_t* err)
 {
     using C = I8SplitCfg<TN>;
     extern __shared__ uint8_t smem_raw[];
     uint8_t* const sW = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
     uint8_t* const sA = sW + C::STAGES * C::W_BYTES;
     float* const s_rowscale = reinterpret_cast<float*>(sA + C::STAGES * C::A_BYTES);
-    uint64_t* const full = reinterpret_cast<uint64_t*>(s_rowscale + TN);
+    uint64_t* const full = reinterpret_cast<uint64_t*>(s_rowscale + TN + 4);   // put2 may look one behind TN
     uint64_t* const empty = full + C::STAGES;
     uint64_t* const done = empty + C::STAGES;      // every MMA of this CTA has completed
     uint32_t* const tmem_slot = reinterpret_cast<uint32_t*>(done + 1);
@@ -320,16 +321,24 @@ __global__ void __launch_bounds__(192) gemm_i8_split_kernel(const __grid_constan
     const uint32_t tmem = *tmem_slot;
     if (threadIdx.x == 0) griddep_launch();
 
-    const int n = n0 + (warp & 3) * 32 + lane;                     // the epilogue's channel of this thread
+    // the epilogue: this thread's channel, its group's share of a tile's or a rank's tokens
+    const int n_in = (warp & 3) * 32 + lane, n = n0 + n_in, grp = (warp - 2) >> 2;
     const int tokens = p.M - m0 < TN ? p.M - m0 : TN;
     const bool in = n < p.N;
     float cs = 0.f, bias = 0.f;
     bool ok = true;
     TO* const c = static_cast<TO*>(p.C) + (size_t)m0 * p.ldc + n;
-    const auto value = [&](int acc, int t) {
-        const float v = i8_value(acc, s_rowscale[t], cs, bias);
-        if constexpr (EPI == kEpiBiasGelu) return gelu_pair<false, true>(pk2(v, v), GeluK(1.0f)).x;
-        return v;
+    // the outputs of tokens t and u from their accumulators; a token outside [0, end) is computed and not stored
+    const auto put2 = [&](int acc_t, int t, int acc_u, int u, int end) {
+        float2 v = make_float2(i8_value(acc_t, s_rowscale[t], cs, bias), i8_value(acc_u, s_rowscale[u], cs, bias));
+        if constexpr (EPI == kEpiBiasGelu) v = gelu_pair<false, true>(pk2(v.x, v.y), GeluK(1.0f));
+        TO *ct = c + (size_t)t * p.ldc, *cu = c + (size_t)u * p.ldc;
+        if constexpr (EPI == kEpiResidual) {
+            if (t < end) v.x += *ct;
+            if (u < end) v.y += *cu;
+        }
+        if (t < end) *ct = from_f32<TO>(v.x);
+        if (u < end) *cu = from_f32<TO>(v.y);
     };
     int* const part = reinterpret_cast<int*>(sW);                  // [tokens][128] partial sums
 
@@ -379,37 +388,30 @@ __global__ void __launch_bounds__(192) gemm_i8_split_kernel(const __grid_constan
     } else {
         griddep_wait();
         const int e = threadIdx.x - 64;
-        if (e < tokens) s_rowscale[e] = __ldg(p.rowscale + m0 + e);
+        if (e < TN) s_rowscale[e] = e < tokens ? __ldg(p.rowscale + m0 + e) : 0.f;
         if (in) {
             cs = __ldg(p.colscale + n);
             if (p.bias) bias = __ldg(p.bias + n);
         }
-        named_barrier(1, 128);
+        named_barrier(1, 128 * C::GROUPS);
         ok = __all_sync(0xffffffffu, mbar_wait(done, 0, err, kErrTmemFull));
         tc_fence_after();
+        constexpr int SHARE = TN / C::GROUPS, LD = SHARE < 16 ? SHARE : 16;
         const uint32_t t_lane = tmem + (static_cast<uint32_t>((warp & 3) * 32) << 16);
-        for (int t0 = 0; ok && t0 < tokens; t0 += 16) {
-            uint32_t a[16];
-            tmem_ld_32x32b_x16(t_lane + static_cast<uint32_t>(t0), a);
+#pragma unroll 1
+        for (int t0 = grp * SHARE; ok && t0 < (grp + 1) * SHARE && t0 < tokens; t0 += LD) {
+            uint32_t a[LD];
+            if constexpr (LD == 4) tmem_ld_32x32b_x4(t_lane + static_cast<uint32_t>(t0), a);
+            else if constexpr (LD == 8) tmem_ld_32x32b_x8(t_lane + static_cast<uint32_t>(t0), a);
+            else tmem_ld_32x32b_x16(t_lane + static_cast<uint32_t>(t0), a);
             tmem_ld_wait();
             if (S > 1) {
 #pragma unroll
-                for (int i = 0; i < 16; ++i)
-                    if (t0 + i < tokens) part[(t0 + i) * 128 + (warp & 3) * 32 + lane] = static_cast<int>(a[i]);
+                for (int i = 0; i < LD; ++i) part[(t0 + i) * 128 + n_in] = static_cast<int>(a[i]);
             } else if (in) {
-                float old[16];
-                if constexpr (EPI == kEpiResidual) {
 #pragma unroll
-                    for (int i = 0; i < 16; ++i) old[i] = t0 + i < tokens ? c[(size_t)(t0 + i) * p.ldc] : 0.f;
-                }
-#pragma unroll
-                for (int i = 0; i < 16; ++i) {
-                    if (t0 + i < tokens) {
-                        float v = value(static_cast<int>(a[i]), t0 + i);
-                        if constexpr (EPI == kEpiResidual) v += old[i];
-                        c[(size_t)(t0 + i) * p.ldc] = from_f32<TO>(v);
-                    }
-                }
+                for (int i = 0; i < LD; i += 2)
+                    put2(static_cast<int>(a[i]), t0 + i, static_cast<int>(a[i + 1]), t0 + i + 1, tokens);
             }
         }
     }
@@ -418,28 +420,21 @@ __global__ void __launch_bounds__(192) gemm_i8_split_kernel(const __grid_constan
     if (S > 1) {
         cluster_sync();            // every CTA's partial sums are written
         if (warp >= 2 && ok && in) {
+            // this CTA's share of the tokens, its groups' tokens neighbouring pairs
             const int ta = static_cast<int>(tokens * rank / S), tb = static_cast<int>(tokens * (rank + 1) / S);
-            const uint32_t mine = smem_u32(part) + 4u * static_cast<uint32_t>((warp & 3) * 32 + lane);
-            for (int t = ta; t < tb; t += 4) {
-                int sum[4] = {0, 0, 0, 0};
+            const uint32_t mine = smem_u32(part) + 4u * static_cast<uint32_t>(n_in);
+            for (int t = ta + 2 * grp; t < tb; t += 2 * C::GROUPS) {
+                const int u = t + 1 < TN ? t + 1 : t;     // in the buffer, if not in the share
+                int x = 0, y = 0;
 #pragma unroll
                 for (uint32_t r = 0; r < 8; ++r) {
                     if (r < S) {
                         const uint32_t from = mapa_shared(mine, r);
-#pragma unroll
-                        for (int i = 0; i < 4; ++i)
-                            if (t + i < tb) sum[i] += static_cast<int>(ld_cluster(from + 512u * static_cast<uint32_t>(t + i)));
+                        x += static_cast<int>(ld_cluster(from + 512u * static_cast<uint32_t>(t)));
+                        y += static_cast<int>(ld_cluster(from + 512u * static_cast<uint32_t>(u)));
                     }
                 }
-#pragma unroll
-                for (int i = 0; i < 4; ++i) {
-                    if (t + i < tb) {
-                        float v = value(sum[i], t + i);
-                        TO* at = c + (size_t)(t + i) * p.ldc;
-                        if constexpr (EPI == kEpiResidual) v += *at;
-                        *at = from_f32<TO>(v);
-                    }
-                }
+                put2(x, t, y, t + 1, tb);
             }
         }
         __syncwarp();

@@ -1756,10 +1756,36 @@ struct GemmI8 {
 // The kernels of an int8 product: the choice of `kernel` -1, else what the caller asks for.
 enum I8Kernel : int { kI8Single = 0, kI8Pair = 1, kI8Split = 2 };   // kI8Split + S: the split over S CTAs
 
+// Tiles of the split kernel with TN tokens each.
+static long long i8_split_tiles(const GemmI8& p, int TN) { return ((p.N + 127LL) / 128) * ((p.M + TN - 1) / TN); }
+
+// Tokens a tile of the split kernel: the fewest whose tiles still run all at once (two CTAs an SM), since the epilogue
+// of a tile takes its tokens' time whatever K is (65 x 2,048 x 1,024 with GELU: 4.7 us with 16, 5.0 with 32, 5.5 with 64,
+// 6.4 with 128; 520 x 2,048 x 1,024: 11.2, 6.4, 6.9, 9.1).
+static int pick_i8_tokens(const GemmI8& p, int num_sms)
+{
+    for (int TN : {16, 32, 64})
+        if (i8_split_tiles(p, TN) <= 2 * num_sms) return TN;
+    return 128;
+}
+
+// CTAs that share a tile's K: more while a third of the SMs stay idle and each keeps two 128-byte blocks of K, or while
+// all run at once and each keeps four (16 x 8,192 x 8,192, 64 tiles: 20.2 us alone, 12.8 with 2, 9.6 with 4, 14.9 with 8;
+// 33 x 1,024 x 1,024, 24 tiles: 4.3, 4.4, 3.8, 4.4).
+static int pick_i8_split(long long tiles, int blocks, int num_sms)
+{
+    int S = 1;
+    while (S < 8 && ((3 * tiles * 2 * S <= 2 * num_sms && blocks >= 4 * S) ||
+                     (tiles * 2 * S <= 2 * num_sms && blocks >= 8 * S)))
+        S *= 2;
+    return S;
+}
+
 static int pick_i8_kernel(const GemmI8& p, int num_sms)
 {
-    const long long tiles = ((p.M + 255LL) / 256) * ((p.N + 255) / 256);
-    return tiles >= num_sms / 2 ? kI8Pair : kI8Split;
+    if (i8_split_tiles(p, 64) <= 2 * num_sms) return kI8Split;
+    const long long pairs = ((p.M + 255LL) / 256) * ((p.N + 255) / 256);
+    return pairs >= 2 * num_sms ? kI8Pair : kI8Single;
 }
 
 template <typename TO, int EPI, int TN>
@@ -1777,10 +1803,9 @@ static void launch_gemm_i8_split(const GemmI8& p, const CUtensorMap& mw, long lo
         attr[dev] = true;
     }
     const int n_tiles = (p.N + 127) / 128, blocks = (p.K + 127) / 128;
-    const long long tiles = (long long)n_tiles * ((p.M + TN - 1) / TN);
-    if (split == 0)
-        for (split = 1; split < 8 && tiles * split * 2 <= 2 * num_sms;) split *= 2;
-    while (split > blocks) split /= 2;
+    const long long tiles = i8_split_tiles(p, TN);
+    if (split == 0) split = pick_i8_split(tiles, blocks, num_sms);
+    while (split > blocks) split /= 2;   // a CTA without a block would have nothing to wait for
     if (tiles * split > (1LL << 31) - 1) throw std::runtime_error("cudanet_k_gemm_i8: too many tiles");
     const CUtensorMap ma = make_map(p.A, MapType::U8, p.K, p.M, pitch_a, 128, TN);
     cudaLaunchConfig_t cfg = {};
@@ -1817,10 +1842,12 @@ static void launch_gemm_i8_t(const GemmI8& p, int kernel, cudaStream_t s)
     const CUtensorMap mw = make_map(p.W, MapType::U8, p.K, p.N, pitch(p.ldw, p.K, p.N), 128, kernel == kI8Single ? 256 : 128);
     if (kernel >= kI8Split) {
         const int split = kernel - kI8Split;
-        if (p.M <= 16) launch_gemm_i8_split<TO, EPI, 16>(p, mw, pa, split, sms, err, s);
-        else if (p.M <= 32) launch_gemm_i8_split<TO, EPI, 32>(p, mw, pa, split, sms, err, s);
-        else if (p.M <= 64) launch_gemm_i8_split<TO, EPI, 64>(p, mw, pa, split, sms, err, s);
-        else launch_gemm_i8_split<TO, EPI, 128>(p, mw, pa, split, sms, err, s);
+        switch (pick_i8_tokens(p, sms)) {
+            case 16: launch_gemm_i8_split<TO, EPI, 16>(p, mw, pa, split, sms, err, s); break;
+            case 32: launch_gemm_i8_split<TO, EPI, 32>(p, mw, pa, split, sms, err, s); break;
+            case 64: launch_gemm_i8_split<TO, EPI, 64>(p, mw, pa, split, sms, err, s); break;
+            default: launch_gemm_i8_split<TO, EPI, 128>(p, mw, pa, split, sms, err, s);
+        }
         return;
     }
     const CUtensorMap ma = make_map(p.A, MapType::U8, p.K, p.M, pa, 128, 128);
