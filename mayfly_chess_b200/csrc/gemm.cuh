@@ -1,8 +1,7 @@
 // The trunk's and the heads' matrix products on the 5th-generation tensor cores (tcgen05, sm_100a).
 //
 //   C[M, N] = A[M, K] * W[N, K]^T  (+ epilogue), A and W 16-bit (f16 or bf16, kind::f16) or e4m3 (the FP8
-//   path, kind::f8f6f4, the accumulator scaled per column in the epilogue), K-major, f32 accumulation; or int8
-//   (kind::i8, s32 accumulation, scaled per row and column; int8.cuh).
+//   path, kind::f8f6f4, the accumulator scaled per column in the epilogue), K-major, f32 accumulation.
 //
 // These are the five products of mayfly/chess/cudanet/cudanet_spec.h:94-101 (qkv, out, ff1, ff2, heads), which
 // the reference runs through cuBLASLt (cudanet/gemm.cpp:209-231) or mma.sync (cudanet/kernels_gemm.cu:99-302).
@@ -48,8 +47,6 @@
 #include <cuda_fp16.h>
 #include <cuda_fp8.h>
 
-#include <type_traits>
-
 #include "ptx.cuh"
 
 // Epilogue groups and staging buffers per group of the f32 residual (added into X by TMA reductions).
@@ -81,40 +78,34 @@ enum Epi : int { kEpiBias = 0, kEpiBiasGelu = 1, kEpiResidual = 2, kEpiF32 = 3, 
 // the FP8 qkv product, slower on the 16-bit products and the residuals' reduce-adds, measured).
 __host__ __device__ constexpr int store_rows(int epi, bool f8) { return epi == kEpiBias && f8 ? 32 : 128; }
 
-// Operand types: 16-bit (kind::f16), e4m3 (kind::f8f6f4) or int8 (kind::i8). A stage row is always 128 bytes (the
-// swizzle atom), so a stage of bytes (F8: e4m3 or int8) holds 128 elements of K and each MMA instruction 32 (16 for
-// 16-bit); the byte sizes, smem descriptors and the 32-byte step per instruction are the same.
+// Operand types: 16-bit (kind::f16) or e4m3 (kind::f8f6f4). A stage row is always 128 bytes (the swizzle atom),
+// so an FP8 stage holds 128 elements of K and each MMA instruction 32 (16 for 16-bit); the byte sizes, smem
+// descriptors and the 32-byte step per instruction are the same.
 template <typename T> struct Operand;
 template <> struct Operand<__half> {
-    static constexpr bool F8 = false, I8 = false;
+    static constexpr bool F8 = false;
     __host__ __device__ static constexpr uint32_t idesc(uint32_t M, uint32_t N) { return idesc_f16(0, M, N); }
 };
 template <> struct Operand<__nv_bfloat16> {
-    static constexpr bool F8 = false, I8 = false;
+    static constexpr bool F8 = false;
     __host__ __device__ static constexpr uint32_t idesc(uint32_t M, uint32_t N) { return idesc_f16(1, M, N); }
 };
 template <> struct Operand<__nv_fp8_e4m3> {
-    static constexpr bool F8 = true, I8 = false;
+    static constexpr bool F8 = true;
     __host__ __device__ static constexpr uint32_t idesc(uint32_t M, uint32_t N) { return idesc_e4m3(M, N); }
-};
-template <> struct Operand<int8_t> {
-    static constexpr bool F8 = true, I8 = true;
-    __host__ __device__ static constexpr uint32_t idesc(uint32_t M, uint32_t N) { return idesc_i8(M, N); }
 };
 
 template <typename TI>
 __device__ __forceinline__ void umma_issue(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc, uint32_t acc)
 {
-    if constexpr (Operand<TI>::I8) umma_i8(d, a, b, idesc, acc);
-    else if constexpr (Operand<TI>::F8) umma_f8(d, a, b, idesc, acc);
+    if constexpr (Operand<TI>::F8) umma_f8(d, a, b, idesc, acc);
     else umma_f16(d, a, b, idesc, acc);
 }
 
 template <typename TI>
 __device__ __forceinline__ void umma_issue_pair(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc, uint32_t acc)
 {
-    if constexpr (Operand<TI>::I8) umma_i8_pair(d, a, b, idesc, acc);
-    else if constexpr (Operand<TI>::F8) umma_f8_pair(d, a, b, idesc, acc);
+    if constexpr (Operand<TI>::F8) umma_f8_pair(d, a, b, idesc, acc);
     else umma_f16_pair(d, a, b, idesc, acc);
 }
 
@@ -125,14 +116,11 @@ struct EpiArgs {
     const float* colscale;   // nullptr: no scaling (16-bit operands)
     float out_scale_inv;     // kEpiGeluE4m3 only
     int rev;                 // 1: the M blocks in descending order (the output is the same)
-    // int8 products only
-    const float* rowscale;   // [M]
 };
 
 // PAIR: the CTA-pair kernel, where a CTA loads BN/2 rows of W per stage and a pair covers 256 rows of M.
-// F8: byte operands (128 elements of K per stage instead of 64; the same bytes). I8: they are int8.
-template <int BN_, int EPI, bool PAIR = false, bool F8 = false, bool I8 = false> struct GemmCfg {
-    static constexpr int BN = BN_;
+// F8: e4m3 operands (128 elements of K per stage instead of 64; the same bytes).
+template <int BN, int EPI, bool PAIR = false, bool F8 = false> struct GemmCfg {
     static constexpr int BM = 128;                      // rows of A and of the output per CTA
     static constexpr int BK = F8 ? 128 : 64;            // elements of K per stage: one 128-byte swizzle row
     static constexpr int KSTEPS = 4;                    // MMA instructions per stage (K = 16 or 32 each, 32 bytes)
@@ -140,7 +128,7 @@ template <int BN_, int EPI, bool PAIR = false, bool F8 = false, bool I8 = false>
     // the residuals are added into X by a TMA reduction at L2 (f32 adds for the f32 stream, bf16 adds of the
     // bf16-rounded v for the bf16 stream), so X is neither read into the SM nor staged
     static constexpr bool REDUCE = EPI == kEpiResidual || EPI == kEpiResidual16;
-    static constexpr bool IS_F8 = F8, IS_I8 = I8;
+    static constexpr bool IS_F8 = F8;
     static constexpr bool HEAVY = EPI == kEpiBiasGelu || EPI == kEpiGeluE4m3;   // GELU's erf per element
     static constexpr int OUT_BYTES = (EPI == kEpiResidual || EPI == kEpiF32) ? 4 : (EPI == kEpiGeluE4m3 ? 1 : 2);
     // one staging chunk: 128 rows x ROW_BYTES (64-byte rows for the GELU epilogues, whose four groups each take
@@ -149,7 +137,7 @@ template <int BN_, int EPI, bool PAIR = false, bool F8 = false, bool I8 = false>
     // product, no faster on the 16-bit one; 128-byte rows otherwise)
     static constexpr bool F8_BIAS = EPI == kEpiBias && F8;
     static constexpr bool NARROW = (F8_BIAS && MF_F8_BIAS_NARROW) || EPI == kEpiResidual16;
-    static constexpr int ROW_BYTES = (HEAVY || NARROW) && !I8 ? 64 : 128;
+    static constexpr int ROW_BYTES = (HEAVY || NARROW) ? 64 : 128;
     static constexpr int STORE_ROWS = store_rows(EPI, F8);   // 32: per-warp stores
     static constexpr int CHUNK_COLS = ROW_BYTES / OUT_BYTES;
     static constexpr int NC = BN / CHUNK_COLS;           // staging chunks per tile
@@ -159,23 +147,22 @@ template <int BN_, int EPI, bool PAIR = false, bool F8 = false, bool I8 = false>
     // issue slots) and for the narrow chunks, two where the chunks are many. The f32 residual stages only
     // acc + bias for its TMA reductions: two groups of one buffer (measured best of 1 x 2, 2 x 1, 2 x 2 and
     // 4 x 1).
-    static constexpr int EG = I8 ? (OUT_BYTES == 4 ? 2 : 4) : EPI == kEpiResidual ? ((NC % MF_REDUCE_EG == 0) ? MF_REDUCE_EG : 1)
+    static constexpr int EG = EPI == kEpiResidual ? ((NC % MF_REDUCE_EG == 0) ? MF_REDUCE_EG : 1)
                               : ((HEAVY || NARROW) && NC % 4 == 0) ? 4 : (NC % 2 == 0 ? 2 : 1);
     // the FP8 bias epilogue with several chunks a group (MF_EPI_BATCH): one staging buffer per chunk, so a group
     // writes all its chunks of a tile before one proxy fence and one barrier, then stores them
     static constexpr bool BATCH = MF_EPI_BATCH && F8_BIAS && NC / EG > 1;
-    static constexpr int NBUF = I8 ? (OUT_BYTES == 4 ? 2 : 1) : BATCH ? NC / EG
+    static constexpr int NBUF = BATCH ? NC / EG
                                 : EPI == kEpiResidual ? MF_REDUCE_NBUF
                                 : F8_BIAS ? MF_F8_BIAS_NBUF : (EG >= 2 ? 1 : 2);   // staging buffers a group
     static constexpr uint32_t A_BYTES = BM * 128;
     static constexpr uint32_t B_BYTES = B_ROWS * 128;
     static constexpr uint32_t STAGE_BYTES = A_BYTES + B_BYTES;
-    static constexpr int VEC_BYTES = I8 ? 2 * 2 * 4 * BN : 0;   // int8: two tiles' column scales and bias
-    static constexpr int STAGES_FIT = (224 * 1024 - EG * NBUF * (int)CHUNK_BYTES - VEC_BYTES) / (int)STAGE_BYTES;
+    static constexpr int STAGES_FIT = (224 * 1024 - EG * NBUF * (int)CHUNK_BYTES) / (int)STAGE_BYTES;
     static constexpr int STAGES = STAGES_FIT > 8 ? 8 : STAGES_FIT;
     static constexpr uint32_t TMEM_COLS = 2 * BN < 32 ? 32 : 2 * BN;
     static constexpr size_t SMEM =
-        1024 + (size_t)STAGES * STAGE_BYTES + (size_t)EG * NBUF * CHUNK_BYTES + VEC_BYTES + 256;
+        1024 + (size_t)STAGES * STAGE_BYTES + (size_t)EG * NBUF * CHUNK_BYTES + 256;
     static constexpr int THREADS = 64 + 128 * EG;
     static_assert(STAGES >= 3, "pipeline too shallow");
     static_assert(SMEM <= 232448, "shared memory over the per-block limit");
@@ -341,13 +328,6 @@ __device__ __forceinline__ void scale_bias32(float (&v)[NV], int off, const floa
     }
 }
 
-// The int8 products' value of one accumulator before GELU or a residual's addition, a rounding a step and the same in
-// every kernel, so that they agree to the bit.
-__device__ __forceinline__ float i8_value(int acc, float rowscale, float colscale, float bias)
-{
-    return fmaf(__fmul_rn(__int2float_rn(acc), rowscale), colscale, bias);
-}
-
 // four floats to four e4m3 bytes (round to nearest even, saturating to +-448), first value in the lowest byte
 __device__ __forceinline__ uint32_t pack_e4m3x4(float a, float b, float c, float d)
 {
@@ -381,7 +361,7 @@ template <typename C> struct SmemLayout {
         sA = smem;
         sB = smem + C::STAGES * C::A_BYTES;
         sC = sB + C::STAGES * C::B_BYTES;                                // EG x NBUF staging chunks
-        full = reinterpret_cast<uint64_t*>(sC + C::EG * C::NBUF * C::CHUNK_BYTES + C::VEC_BYTES);
+        full = reinterpret_cast<uint64_t*>(sC + C::EG * C::NBUF * C::CHUNK_BYTES);
         empty = full + C::STAGES;
         tfull = empty + C::STAGES;
         tempty = tfull + 2;
@@ -549,133 +529,14 @@ __device__ __forceinline__ void epilogue_loop(const SmemLayout<C>& L, const CUte
     if (C::STORE_ROWS == 32 ? lane == 0 : leader) bulk_wait_all();
 }
 
-// The epilogue of the int8 products. A warp owns 32 rows of the tile and COLS neighbouring columns of them: it converts
-// them from tensor memory into its own staging chunk of 32 rows x 128 bytes, and its lane 0 stores the chunk (for the
-// residual: adds it at L2) by TMA, so that the warps of a group meet once a tile and not at every chunk. The group's
-// column scales and bias of a tile are read by its 128 threads a tile ahead and passed through shared memory: each is
-// read once from L2, and an aligned float4 serves a warp.
-template <typename TO, int EPI, typename C, typename RowFn, typename ColFn, typename ReleaseFn>
-__device__ __forceinline__ void epilogue_loop_i8(const SmemLayout<C>& L, const CUtensorMap* tmC, uint32_t tmem_base,
-                                                 int my_tiles, RowFn origin_row, ColFn origin_col, ReleaseFn release,
-                                                 const EpiArgs& ep, int M, int N, uint32_t* err)
-{
-    griddep_wait();
-    constexpr int COLS = C::BN / C::EG;               // columns of a group
-    constexpr int VECS = 2 * COLS;                    // its column scales, then its bias
-    constexpr int PER = VECS / 128;
-    constexpr int CHUNK = C::CHUNK_COLS;              // columns of 128 bytes
-    static_assert(VECS % 128 == 0 && COLS % CHUNK == 0 && C::ROW_BYTES == 128, "a group's columns must be whole chunks");
-    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-    const int grp = (warp - 2) >> 2, gtid = (int)threadIdx.x - 64 - 128 * grp;
-    const int quarter = warp & 3;
-    const int row = quarter * 32 + lane;
-    const uint32_t bar_id = 1 + grp;
-    const uint32_t t_lane = tmem_base + (static_cast<uint32_t>(quarter * 32) << 16) + static_cast<uint32_t>(grp * COLS);
-    uint8_t* const stages = L.sC + (grp * 4 + quarter) * C::NBUF * 4096;
-    float* const svec = reinterpret_cast<float*>(L.sC + C::EG * C::NBUF * C::CHUNK_BYTES) + grp * 2 * VECS;
-    int chunk = 0;
-
-    float next[PER], next_rs = 0.f;
-    auto read_ahead = [&](int it) {
-        if (it >= my_tiles) return;
-        const int col0 = origin_col(it) + grp * COLS, r = origin_row(it) + row;
-#pragma unroll
-        for (int j = 0; j < PER; ++j) {
-            const int k = gtid + 128 * j, n = col0 + (k & (COLS - 1));
-            const float* src = k < COLS ? ep.colscale : ep.bias;
-            next[j] = src && n < N ? __ldg(src + n) : 0.f;
-        }
-        next_rs = r < M ? __ldg(ep.rowscale + r) : 0.f;
-    };
-    read_ahead(0);
-
-    int acc = 0;
-    uint32_t acc_phase = 0;
-    for (int it = 0; it < my_tiles; ++it) {
-        const int row0 = origin_row(it) + quarter * 32, col0 = origin_col(it) + grp * COLS;
-        float* sv = svec + (it & 1) * VECS;           // the other half is still read by this group's slower warps
-#pragma unroll
-        for (int j = 0; j < PER; ++j) sv[gtid + 128 * j] = next[j];
-        const uint64_t rs2 = pk2(next_rs, next_rs);
-        if (gtid == 0) L.epi_ok[grp] = mbar_wait(&L.tfull[acc], acc_phase, err, kErrTmemFull) ? 1u : 0u;
-        named_barrier(bar_id, 128);
-        if (!L.epi_ok[grp]) break;
-        tc_fence_after();
-        read_ahead(it + 1);
-        const uint32_t t_acc = t_lane + static_cast<uint32_t>(acc * C::BN);
-#pragma unroll 1
-        for (int c = 0; c < COLS; c += CHUNK) {
-            uint32_t q[32];                            // the row's 128 bytes
-#pragma unroll
-            for (int p = 0; p < CHUNK; p += 32) {
-                uint32_t a[32];
-                tmem_ld_32x32b_x32(t_acc + static_cast<uint32_t>(c + p), a);
-                tmem_ld_wait();
-                if (c + p == COLS - 32) {
-                    tc_fence_before();
-                    __syncwarp();
-                    if (lane == 0) release(acc);
-                }
-#pragma unroll
-                for (int i = 0; i < 32; i += 4) {
-                    const float4 sc = *reinterpret_cast<const float4*>(sv + c + p + i);
-                    const float4 b = *reinterpret_cast<const float4*>(sv + COLS + c + p + i);
-                    const uint64_t lo = fma2(mul2(pk2(__int2float_rn((int)a[i]), __int2float_rn((int)a[i + 1])), rs2),
-                                             pk2(sc.x, sc.y), pk2(b.x, b.y));
-                    const uint64_t hi =
-                        fma2(mul2(pk2(__int2float_rn((int)a[i + 2]), __int2float_rn((int)a[i + 3])), rs2),
-                             pk2(sc.z, sc.w), pk2(b.z, b.w));
-                    float2 x, y;
-                    if constexpr (EPI == kEpiBiasGelu) {
-                        const GeluK K(1.0f);
-                        x = gelu_pair<false, true>(lo, K);
-                        y = gelu_pair<false, true>(hi, K);
-                    } else {
-                        x = upk2(lo);
-                        y = upk2(hi);
-                    }
-                    if constexpr (sizeof(TO) == 2) {
-                        q[(p + i) / 2] = pack2<TO>(x.x, x.y);
-                        q[(p + i) / 2 + 1] = pack2<TO>(y.x, y.y);
-                    } else {
-                        q[i] = __float_as_uint(x.x);
-                        q[i + 1] = __float_as_uint(x.y);
-                        q[i + 2] = __float_as_uint(y.x);
-                        q[i + 3] = __float_as_uint(y.y);
-                    }
-                }
-            }
-            uint8_t* stage = stages + (chunk % C::NBUF) * 4096;
-            ++chunk;
-            if (lane == 0) bulk_wait_read<C::NBUF - 1>();   // the last store out of this chunk has read it
-            __syncwarp();
-#pragma unroll
-            for (int j = 0; j < 8; ++j)
-                *reinterpret_cast<uint4*>(stage + swz<128>(lane, j)) =
-                    make_uint4(q[4 * j], q[4 * j + 1], q[4 * j + 2], q[4 * j + 3]);
-            fence_proxy_async_smem();
-            __syncwarp();
-            if (lane == 0 && row0 < M) {
-                if constexpr (EPI == kEpiResidual) tma_reduce_add_2d(tmC, stage, col0 + c, row0);
-                else tma_store_2d(tmC, stage, col0 + c, row0);
-                bulk_commit();
-            }
-        }
-        acc ^= 1;
-        if (acc == 0) acc_phase ^= 1u;
-    }
-    if (lane == 0) bulk_wait_all();
-}
-
 // ------------------------------------------------------------------------------------------------ one CTA
-// TI: the operands' type (f16, bf16, e4m3 or int8); T: the 16-bit output type of kEpiBias / kEpiBiasGelu (int8: the
-// output's type, f32 among them).
+// TI: the operands' type (f16, bf16 or e4m3); T: the 16-bit output type of kEpiBias / kEpiBiasGelu.
 template <typename TI, typename T, int BN, int EPI>
-__global__ void __launch_bounds__(GemmCfg<BN, EPI, false, Operand<TI>::F8, Operand<TI>::I8>::THREADS, 1)
+__global__ void __launch_bounds__(GemmCfg<BN, EPI, false, Operand<TI>::F8>::THREADS, 1)
 gemm_tc_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant__ CUtensorMap tmB,
                const __grid_constant__ CUtensorMap tmC, int M, int N, int K, const EpiArgs ep, uint32_t* err)
 {
-    using C = GemmCfg<BN, EPI, false, Operand<TI>::F8, Operand<TI>::I8>;
+    using C = GemmCfg<BN, EPI, false, Operand<TI>::F8>;
     extern __shared__ uint8_t smem_raw[];
     const SmemLayout<C> L(smem_raw);
 
@@ -683,7 +544,7 @@ gemm_tc_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant__ 
     const int m_tiles = (M + C::BM - 1) / C::BM;
     const int n_tiles = (N + BN - 1) / BN;
     const int num_tiles = m_tiles * n_tiles;
-    const int k_iters = C::IS_I8 ? (K + C::BK - 1) / C::BK : K / C::BK;   // int8: TMA fills K's tail with zeros
+    const int k_iters = K / C::BK;
 
     if (threadIdx.x == 0) {
         for (int s = 0; s < C::STAGES; ++s) {
@@ -720,8 +581,7 @@ gemm_tc_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant__ 
             bool ok = true;
             // the weight tiles of this CTA's first stages depend on no earlier kernel: they load while that
             // kernel finishes; A (an earlier kernel's output) only after griddep_wait
-            // (int8 products are queued by themselves: the kernel before one may write its weights)
-            const int pre = !C::IS_I8 && (int)blockIdx.x < num_tiles ? (k_iters < C::STAGES ? k_iters : C::STAGES) : 0;
+            const int pre = (int)blockIdx.x < num_tiles ? (k_iters < C::STAGES ? k_iters : C::STAGES) : 0;
             for (int kb = 0; kb < pre; ++kb) {
                 mbar_arrive_expect_tx(&L.full[kb], C::STAGE_BYTES);
                 tma_load_2d(L.sB + kb * C::B_BYTES, &tmB, &L.full[kb], kb * C::BK, ((int)blockIdx.x % n_tiles) * BN);
@@ -795,16 +655,14 @@ gemm_tc_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant__ 
     } else if (k_iters > 0) {
         const int my_tiles =
             (int)blockIdx.x < num_tiles ? (num_tiles - 1 - (int)blockIdx.x) / (int)gridDim.x + 1 : 0;
-        const auto origin_row = [&](int it) {
-            const int m_fwd = ((int)blockIdx.x + it * (int)gridDim.x) / n_tiles;
-            return (ep.rev ? m_tiles - 1 - m_fwd : m_fwd) * C::BM;
-        };
-        const auto origin_col = [&](int it) { return (((int)blockIdx.x + it * (int)gridDim.x) % n_tiles) * BN; };
-        const auto release = [&](int acc) { mbar_arrive(&L.tempty[acc]); };
-        if constexpr (C::IS_I8)
-            epilogue_loop_i8<T, EPI, C>(L, &tmC, tmem_base, my_tiles, origin_row, origin_col, release, ep, M, N, err);
-        else
-            epilogue_loop<T, EPI, C>(L, &tmC, tmem_base, my_tiles, origin_row, origin_col, release, ep, M, N, err);
+        epilogue_loop<T, EPI, C>(
+            L, &tmC, tmem_base, my_tiles,
+            [&](int it) {
+                const int m_fwd = ((int)blockIdx.x + it * (int)gridDim.x) / n_tiles;
+                return (ep.rev ? m_tiles - 1 - m_fwd : m_fwd) * C::BM;
+            },
+            [&](int it) { return (((int)blockIdx.x + it * (int)gridDim.x) % n_tiles) * BN; },
+            [&](int acc) { mbar_arrive(&L.tempty[acc]); }, ep, M, N, err);
     }
 
     __syncwarp();
@@ -819,12 +677,12 @@ gemm_tc_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant__ 
 // CTAs' loads complete there), the accumulator's `tempty` barriers (both CTAs' epilogue warps arrive there) and
 // issues every MMA; each CTA's `empty` and `tfull` barriers are signalled by the leader's commits.
 template <typename TI, typename T, int EPI>
-__global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(GemmCfg<256, EPI, true, Operand<TI>::F8, Operand<TI>::I8>::THREADS, 1)
+__global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(GemmCfg<256, EPI, true, Operand<TI>::F8>::THREADS, 1)
 gemm_tc_pair_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant__ CUtensorMap tmB,
                     const __grid_constant__ CUtensorMap tmC, int M, int N, int K, const EpiArgs ep, uint32_t* err)
 {
     constexpr int BN = 256;
-    using C = GemmCfg<BN, EPI, true, Operand<TI>::F8, Operand<TI>::I8>;
+    using C = GemmCfg<BN, EPI, true, Operand<TI>::F8>;
     extern __shared__ uint8_t smem_raw[];
     const SmemLayout<C> L(smem_raw);
 
@@ -835,7 +693,7 @@ gemm_tc_pair_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_consta
     const int m_tiles = (M + 2 * C::BM - 1) / (2 * C::BM);
     const int n_tiles = (N + BN - 1) / BN;
     const int num_tiles = m_tiles * n_tiles;
-    const int k_iters = C::IS_I8 ? (K + C::BK - 1) / C::BK : K / C::BK;   // int8: TMA fills K's tail with zeros
+    const int k_iters = K / C::BK;
 
     if (threadIdx.x == 0) {
         for (int s = 0; s < C::STAGES; ++s) {
@@ -870,7 +728,7 @@ gemm_tc_pair_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_consta
             uint32_t issued = 0, issued_par = 0;
             bool ok = true;
             // this CTA's half of the first stages' weight tiles loads before griddep_wait (as in gemm_tc_kernel)
-            const int pre = !C::IS_I8 && pair < num_tiles ? (k_iters < C::STAGES ? k_iters : C::STAGES) : 0;
+            const int pre = pair < num_tiles ? (k_iters < C::STAGES ? k_iters : C::STAGES) : 0;
             for (int kb = 0; kb < pre; ++kb) {
                 if (lead) mbar_arrive_expect_tx(&L.full[kb], 2 * C::STAGE_BYTES);
                 tma_load_2d_pair(L.sB + kb * C::B_BYTES, &tmB, mapa_shared(smem_u32(&L.full[kb]), 0), kb * C::BK,
@@ -957,20 +815,14 @@ gemm_tc_pair_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_consta
         const int my_tiles = pair < num_tiles ? (num_tiles - 1 - pair) / num_pairs + 1 : 0;
         const uint32_t tempty_lead0 = mapa_shared(smem_u32(&L.tempty[0]), 0);
         const uint32_t tempty_lead1 = mapa_shared(smem_u32(&L.tempty[1]), 0);
-        const auto origin_row = [&](int it) {
-            const int m_fwd = (pair + it * num_pairs) / n_tiles;
-            return (ep.rev ? m_tiles - 1 - m_fwd : m_fwd) * 2 * C::BM + (int)rank * C::BM;
-        };
-        const auto origin_col = [&](int it) { return ((pair + it * num_pairs) % n_tiles) * BN; };
-        const auto release = [&](int acc) {
-            const uint32_t bar = acc ? tempty_lead1 : tempty_lead0;
-            if constexpr (C::IS_I8) mbar_arrive_cluster_tmem(bar);
-            else mbar_arrive_cluster(bar);
-        };
-        if constexpr (C::IS_I8)
-            epilogue_loop_i8<T, EPI, C>(L, &tmC, tmem_base, my_tiles, origin_row, origin_col, release, ep, M, N, err);
-        else
-            epilogue_loop<T, EPI, C>(L, &tmC, tmem_base, my_tiles, origin_row, origin_col, release, ep, M, N, err);
+        epilogue_loop<T, EPI, C>(
+            L, &tmC, tmem_base, my_tiles,
+            [&](int it) {
+                const int m_fwd = (pair + it * num_pairs) / n_tiles;
+                return (ep.rev ? m_tiles - 1 - m_fwd : m_fwd) * 2 * C::BM + (int)rank * C::BM;
+            },
+            [&](int it) { return ((pair + it * num_pairs) % n_tiles) * BN; },
+            [&](int acc) { mbar_arrive_cluster(acc ? tempty_lead1 : tempty_lead0); }, ep, M, N, err);
     }
 
     __syncwarp();

@@ -253,6 +253,304 @@ __global__ void __launch_bounds__(L ? 256 : 1024) rows_i8_kernel(const RowsI8 a)
     }
 }
 
+// The value of an accumulator before GELU or a residual's addition, a rounding a step and the same in every kernel, so
+// that they agree to the bit.
+__device__ __forceinline__ float i8_value(int acc, float rowscale, float colscale, float bias)
+{
+    return fmaf(__fmul_rn(__int2float_rn(acc), rowscale), colscale, bias);
+}
+
+// The outputs and vectors of a product.
+struct I8Out {
+    const float *rowscale, *colscale, *bias;
+    void* C;
+    long long ldc;
+    int M, N, K, n_tiles;
+};
+
+// ------------------------------------------------------------------------------------------------ many rows
+// 256 x 256 tiles on CTA pairs (tcgen05.mma.cta_group::2, kind::i8), persistent: each CTA holds 128 rows of A, 128 of the
+// 256 rows of W and 128 x 256 accumulators, two of them, so that a tile's epilogue runs under the next tile's products.
+// What bounds it is shared memory's bandwidth: at the full rate of the products the operands' arrival takes half of the
+// 128 bytes a cycle and their reading the other half, and the epilogue's staging comes on top. So a pair takes
+// neighbouring tiles, W's blocks fastest, and keeps its rows of A in shared memory over all of them where they fit
+// (K <= 1,024): only W then streams. Roles: warp 0 TMA loads, warp 1 tensor memory and the products (leader CTA),
+// warps 2..17 the epilogue.
+struct I8PairCfg {
+    static constexpr int SLOTS = 11;                     // of 128 rows x 128 bytes
+    static constexpr uint32_t SLOT = 128 * 128;
+    static constexpr int MAX_A = 8, RING = 5;            // blocks of A that stay; stages of both where they do not
+    static constexpr int MAX_B = 8;
+    static constexpr int GROUPS = 4, COLS = 64;          // epilogue groups of 4 warps, columns of a tile each
+    static constexpr uint32_t STAGE = 32 * 64;           // a warp's staging: 32 rows x 64 bytes
+    static constexpr size_t SMEM = 1024 + SLOTS * SLOT + 4 * GROUPS * STAGE + GROUPS * 2 * 2 * COLS * 4 + 512;
+    static constexpr int THREADS = 64 + 128 * GROUPS;
+};
+
+// A warp owns 32 rows of the tile and COLS neighbouring columns: it converts them from tensor memory into its own
+// staging chunk, and its lane 0 stores the chunk (for the residual: adds it at L2) by TMA, so that the warps of a group
+// meet once a tile and not at every chunk. The group's column scales and bias of a tile are read by its 128 threads a
+// tile ahead and passed through shared memory: each is read once from L2, and an aligned float4 serves a warp.
+template <typename TO, int EPI, typename OriginFn, typename ReleaseFn>
+__device__ __forceinline__ void i8_pair_epilogue(const CUtensorMap* tmC, const I8Out& p, uint8_t* stages, float* vecs,
+                                                 volatile uint32_t* epi_ok, uint64_t* tfull, uint32_t tmem_base,
+                                                 int tiles, OriginFn origin, ReleaseFn release, uint32_t* err)
+{
+    using C = I8PairCfg;
+    griddep_wait();
+    constexpr int COLS = C::COLS, CHUNK = 64 / sizeof(TO);   // columns of a 64-byte row of staging
+    constexpr int LD = CHUNK < 32 ? CHUNK : 32;
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    const int grp = (warp - 2) >> 2, gtid = (int)threadIdx.x - 64 - 128 * grp;
+    const int quarter = warp & 3;
+    const uint32_t t_lane = tmem_base + (static_cast<uint32_t>(quarter * 32) << 16) + static_cast<uint32_t>(grp * COLS);
+    uint8_t* const stage = stages + (grp * 4 + quarter) * C::STAGE;
+    float* const svec = vecs + grp * 2 * 2 * COLS;
+
+    float next = 0.f, next_rs = 0.f;
+    auto read_ahead = [&](int it) {
+        if (it >= tiles) return;
+        const int2 o = origin(it);                           // row, column
+        const int n = o.y + grp * COLS + (gtid & (COLS - 1)), r = o.x + quarter * 32 + lane;
+        const float* src = gtid < COLS ? p.colscale : p.bias;
+        next = src && n < p.N ? __ldg(src + n) : 0.f;
+        next_rs = r < p.M ? __ldg(p.rowscale + r) : 0.f;
+    };
+    read_ahead(0);
+
+    int acc = 0;
+    uint32_t acc_phase = 0;
+    for (int it = 0; it < tiles; ++it) {
+        const int2 o = origin(it);
+        const int row0 = o.x + quarter * 32, col0 = o.y + grp * COLS;
+        float* sv = svec + (it & 1) * 2 * COLS;              // the other half is still read by this group's slower warps
+        sv[gtid] = next;
+        const uint64_t rs2 = pk2(next_rs, next_rs);
+        if (gtid == 0) epi_ok[grp] = mbar_wait(&tfull[acc], acc_phase, err, kErrTmemFull) ? 1u : 0u;
+        named_barrier(1 + grp, 128);
+        if (!epi_ok[grp]) break;
+        tc_fence_after();
+        read_ahead(it + 1);
+        const uint32_t t_acc = t_lane + static_cast<uint32_t>(acc * 256);
+#pragma unroll 1
+        for (int c = 0; c < COLS; c += CHUNK) {
+            uint32_t a[LD], q[16];
+            if constexpr (LD == 32) tmem_ld_32x32b_x32(t_acc + static_cast<uint32_t>(c), a);
+            else tmem_ld_32x32b_x16(t_acc + static_cast<uint32_t>(c), a);
+            tmem_ld_wait();
+            if (c == COLS - CHUNK) {
+                tc_fence_before();
+                __syncwarp();
+                if (lane == 0) release(acc);
+            }
+#pragma unroll
+            for (int i = 0; i < LD; i += 4) {
+                const float4 sc = *reinterpret_cast<const float4*>(sv + c + i);
+                const float4 b = *reinterpret_cast<const float4*>(sv + COLS + c + i);
+                const uint64_t lo = fma2(mul2(pk2(__int2float_rn((int)a[i]), __int2float_rn((int)a[i + 1])), rs2),
+                                         pk2(sc.x, sc.y), pk2(b.x, b.y));
+                const uint64_t hi = fma2(mul2(pk2(__int2float_rn((int)a[i + 2]), __int2float_rn((int)a[i + 3])), rs2),
+                                         pk2(sc.z, sc.w), pk2(b.z, b.w));
+                float2 x, y;
+                if constexpr (EPI == kEpiBiasGelu) {
+                    const GeluK K(1.0f);
+                    x = gelu_pair<false, true>(lo, K);
+                    y = gelu_pair<false, true>(hi, K);
+                } else {
+                    x = upk2(lo);
+                    y = upk2(hi);
+                }
+                if constexpr (sizeof(TO) == 2) {
+                    q[i / 2] = pack2<TO>(x.x, x.y);
+                    q[i / 2 + 1] = pack2<TO>(y.x, y.y);
+                } else {
+                    q[i] = __float_as_uint(x.x);
+                    q[i + 1] = __float_as_uint(x.y);
+                    q[i + 2] = __float_as_uint(y.x);
+                    q[i + 3] = __float_as_uint(y.y);
+                }
+            }
+            if (lane == 0) bulk_wait_read<0>();              // the last store out of this chunk has read it
+            __syncwarp();
+#pragma unroll
+            for (int j = 0; j < 4; ++j)
+                *reinterpret_cast<uint4*>(stage + swz<64>(lane, j)) =
+                    make_uint4(q[4 * j], q[4 * j + 1], q[4 * j + 2], q[4 * j + 3]);
+            fence_proxy_async_smem();
+            __syncwarp();
+            if (lane == 0 && row0 < p.M) {
+                if constexpr (EPI == kEpiResidual) tma_reduce_add_2d(tmC, stage, col0 + c, row0);
+                else tma_store_2d(tmC, stage, col0 + c, row0);
+                bulk_commit();
+            }
+        }
+        acc ^= 1;
+        if (acc == 0) acc_phase ^= 1u;
+    }
+    if (lane == 0) bulk_wait_all();
+}
+
+template <typename TO, int EPI>
+__global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(I8PairCfg::THREADS, 1)
+gemm_i8_pair_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant__ CUtensorMap tmW,
+                    const __grid_constant__ CUtensorMap tmC, const I8Out p, uint32_t* err)
+{
+    using C = I8PairCfg;
+    extern __shared__ uint8_t smem_raw[];
+    uint8_t* const slots = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
+    uint8_t* const stages = slots + C::SLOTS * C::SLOT;
+    float* const vecs = reinterpret_cast<float*>(stages + 4 * C::GROUPS * C::STAGE);
+    uint64_t* const full_a = reinterpret_cast<uint64_t*>(vecs + C::GROUPS * 2 * 2 * C::COLS);
+    uint64_t* const empty_a = full_a + C::MAX_A;
+    uint64_t* const full_b = empty_a + C::MAX_A;
+    uint64_t* const empty_b = full_b + C::MAX_B;
+    uint64_t* const tfull = empty_b + C::MAX_B;
+    uint64_t* const tempty = tfull + 2;
+    uint64_t* const mma_done = tempty + 2;
+    uint32_t* const tmem_slot = reinterpret_cast<uint32_t*>(mma_done + 1);
+    volatile uint32_t* const epi_ok = tmem_slot + 1;
+
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    const uint32_t rank = cluster_ctarank();
+    const bool lead = rank == 0;
+    const int pair = (int)blockIdx.x >> 1, pairs = (int)gridDim.x >> 1;
+    const long long all = (long long)((p.M + 255) / 256) * p.n_tiles;
+    const int lo = static_cast<int>(all * pair / pairs), hi = static_cast<int>(all * (pair + 1) / pairs);
+    const int blocks = (p.K + 127) / 128;
+    // A's blocks stay over a row of tiles, in slots of their own; else both operands go round a ring
+    const bool stay = blocks <= C::MAX_A;
+    const int na = stay ? blocks : C::RING;
+    const int nb = stay ? (C::SLOTS - na < C::MAX_B ? C::SLOTS - na : C::MAX_B) : C::RING;
+
+    if (threadIdx.x == 0) {
+        for (int s = 0; s < C::MAX_A; ++s) {
+            mbar_init(&full_a[s], 1);
+            mbar_init(&empty_a[s], 1);
+        }
+        for (int s = 0; s < C::MAX_B; ++s) {
+            mbar_init(&full_b[s], 1);
+            mbar_init(&empty_b[s], 1);
+        }
+        for (int b = 0; b < 2; ++b) {
+            mbar_init(&tfull[b], 1);
+            mbar_init(&tempty[b], 2 * 4 * C::GROUPS);   // the epilogue warps of both CTAs
+        }
+        mbar_init(mma_done, 1);
+        fence_barrier_init();
+        tma_prefetch_desc(&tmA);
+        tma_prefetch_desc(&tmW);
+        tma_prefetch_desc(&tmC);
+    }
+    if (warp == 1) {
+        tmem_alloc_pair(tmem_slot, 512);
+        tmem_relinquish_pair();
+    }
+    tc_fence_before();
+    cluster_sync();   // both CTAs' barriers exist before either signals the other's
+    tc_fence_after();
+    const uint32_t tmem_base = *tmem_slot;
+    if (threadIdx.x == 0) griddep_launch();
+
+    if (warp == 0) {
+        if (lane == 0) {
+            griddep_wait();
+            int sa = 0, sb = 0;
+            uint32_t pha = 0, phb = 0;                  // parities of the rounds of A's and W's slots
+            uint32_t used_a = 0, par_a = 0, used_b = 0, par_b = 0;   // slots loaded, and the parity of their last load
+            bool ok = true;
+            for (int tile = lo; tile < hi && ok; ++tile) {
+                const int n_blk = tile % p.n_tiles;
+                const int a_row = tile / p.n_tiles * 256 + (int)rank * 128, b_row = n_blk * 256 + (int)rank * 128;
+                const bool fresh = stay && (tile == lo || n_blk == 0);
+                for (int kb = 0; kb < blocks; ++kb) {
+                    if (fresh) {
+                        if (!(ok = mbar_wait(&empty_a[sa], pha ^ 1u, err, kErrSmemEmpty))) break;
+                        if (lead) mbar_arrive_expect_tx(&full_a[sa], 2 * C::SLOT);
+                        tma_load_2d_pair(slots + sa * C::SLOT, &tmA, mapa_shared(smem_u32(&full_a[sa]), 0), kb * 128, a_row);
+                        used_a |= 1u << sa;
+                        par_a = (par_a & ~(1u << sa)) | (pha << sa);
+                        if (++sa == na) sa = 0, pha ^= 1u;
+                    }
+                    if (!(ok = mbar_wait(&empty_b[sb], phb ^ 1u, err, kErrSmemEmpty))) break;
+                    if (lead) mbar_arrive_expect_tx(&full_b[sb], (stay ? 2 : 4) * C::SLOT);
+                    const uint32_t full = mapa_shared(smem_u32(&full_b[sb]), 0);
+                    if (!stay) tma_load_2d_pair(slots + sb * C::SLOT, &tmA, full, kb * 128, a_row);
+                    tma_load_2d_pair(slots + (na + sb) * C::SLOT, &tmW, full, kb * 128, b_row);
+                    used_b |= 1u << sb;
+                    par_b = (par_b & ~(1u << sb)) | (phb << sb);
+                    if (++sb == nb) sb = 0, phb ^= 1u;
+                }
+            }
+            // this CTA's copies have landed before it can leave: the leader sees them on its `full` barriers, the other
+            // CTA on its `empty` ones (a slot is released only after both halves landed and were read)
+            for (int s = 0; s < C::MAX_A; ++s)
+                if (used_a >> s & 1) mbar_wait(lead ? &full_a[s] : &empty_a[s], par_a >> s & 1, err, kErrTmaFull);
+            for (int s = 0; s < C::MAX_B; ++s)
+                if (used_b >> s & 1) mbar_wait(lead ? &full_b[s] : &empty_b[s], par_b >> s & 1, err, kErrTmaFull);
+        }
+    } else if (warp == 1) {
+        if (lead) {
+            // The whole warp walks the loop and one lane issues, so that stages and descriptors stay in uniform
+            // registers: issuing is what paces the products otherwise.
+            constexpr uint32_t idesc = idesc_i8(256, 256);
+            const uint64_t desc0 = sdesc_sw128(smem_u32(slots));
+            int sb = 0;
+            uint32_t pha = 0, phb = 0;
+            int acc = 0, n_blk = lo % p.n_tiles;
+            uint32_t acc_phase = 0;
+            bool ok = true;
+            for (int tile = lo; tile < hi; ++tile) {
+                if (!__all_sync(0xffffffffu, mbar_wait(&tempty[acc], acc_phase ^ 1u, err, kErrTmemEmpty))) break;
+                tc_fence_after();
+                const bool fresh = stay && (tile == lo || n_blk == 0);
+                const bool last = stay && (tile == hi - 1 || n_blk == p.n_tiles - 1);
+                const uint32_t d = tmem_base + static_cast<uint32_t>(acc * 256);
+                for (int kb = 0; kb < blocks; ++kb) {
+                    ok = !fresh || mbar_wait(&full_a[kb], pha, err, kErrTmaFull);
+                    ok = mbar_wait(&full_b[sb], phb, err, kErrTmaFull) && ok;
+                    if (!(ok = __all_sync(0xffffffffu, ok))) break;
+                    tc_fence_after();
+                    // a slot is SLOT / 16 steps of a descriptor's address, an instruction's 32 bytes of K two
+                    const uint64_t a = desc0 + static_cast<uint32_t>((stay ? kb : sb) * (int)(C::SLOT / 16));
+                    const uint64_t w = desc0 + static_cast<uint32_t>((na + sb) * (int)(C::SLOT / 16));
+                    if (elect_one()) {
+#pragma unroll
+                        for (int k = 0; k < 4; ++k) umma_i8_pair(d, a + 2 * k, w + 2 * k, idesc, (kb | k) != 0 ? 1u : 0u);
+                        umma_commit_pair_both(&empty_b[sb]);
+                        if (last) umma_commit_pair_both(&empty_a[kb]);
+                        if (kb == blocks - 1) umma_commit_pair_both(&tfull[acc]);
+                    }
+                    __syncwarp();
+                    if (++sb == nb) sb = 0, phb ^= 1u;
+                }
+                if (!ok) break;
+                if (last) pha ^= 1u;
+                if (++n_blk == p.n_tiles) n_blk = 0;
+                acc ^= 1;
+                if (acc == 0) acc_phase ^= 1u;
+            }
+            // every product issued has completed (both CTAs' tensor memory) before either frees it
+            if (elect_one()) umma_commit_pair(smem_u32(mma_done));
+            __syncwarp();
+            mbar_wait(mma_done, 0, err, kErrTmemFull);
+        }
+    } else {
+        const uint32_t tempty0 = mapa_shared(smem_u32(&tempty[0]), 0), tempty1 = mapa_shared(smem_u32(&tempty[1]), 0);
+        i8_pair_epilogue<TO, EPI>(
+            &tmC, p, stages, vecs, epi_ok, tfull, tmem_base, hi - lo,
+            [&](int it) {
+                return make_int2((lo + it) / p.n_tiles * 256 + (int)rank * 128, (lo + it) % p.n_tiles * 256);
+            },
+            [&](int acc) { mbar_arrive_cluster_tmem(acc ? tempty1 : tempty0); }, err);
+    }
+
+    __syncwarp();
+    tc_fence_before();
+    cluster_sync();   // the leader's products are done and no CTA signals the other any more
+    tc_fence_after();
+    if (warp == 1) tmem_dealloc_pair(tmem_base, 512);
+}
+
 // ------------------------------------------------------------------------------------------------ few rows
 // The product for few rows of A, and for outputs whose rows are not whole 16-byte units. The weight takes the 128 lanes
 // of the tensor-core instruction (M = 128 rows of W) and the tokens its columns (N = TN rows of A), so that a few tokens
@@ -268,14 +566,6 @@ template <int TN> struct I8SplitCfg {
     static constexpr int GROUPS = 4;                                  // of 4 epilogue warps, TN / 4 tokens each
     static constexpr int THREADS = 64 + 128 * GROUPS;
     static_assert(STAGES * STAGE_BYTES >= 4 * 128 * TN, "the partial sums lie where the stages were");
-};
-
-// The outputs and vectors of a product.
-struct I8Out {
-    const float *rowscale, *colscale, *bias;
-    void* C;
-    long long ldc;
-    int M, N, K, n_tiles;
 };
 
 template <typename TO, int EPI, int TN>

@@ -171,7 +171,7 @@ template <typename TI, typename T, int BN, int EPI>
 static void launch_gemm_bn(const CUtensorMap& ma, const CUtensorMap& mb, const CUtensorMap& mc, int M, int N, int K,
                            const EpiArgs& ep, uint32_t* err, int num_sms, cudaStream_t s)
 {
-    using C = GemmCfg<BN, EPI, false, Operand<TI>::F8, Operand<TI>::I8>;
+    using C = GemmCfg<BN, EPI, false, Operand<TI>::F8>;
     // the shared-memory opt-in, once per instantiation and device (the first launch of a batch size is eager,
     // never inside a graph capture)
     static bool attr[64] = {};
@@ -194,7 +194,7 @@ template <typename TI, typename T, int EPI>
 static void launch_gemm_pair(const CUtensorMap& ma, const CUtensorMap& mb, const CUtensorMap& mc, int M, int N,
                              int K, const EpiArgs& ep, uint32_t* err, cudaStream_t s)
 {
-    using C = GemmCfg<256, EPI, true, Operand<TI>::F8, Operand<TI>::I8>;
+    using C = GemmCfg<256, EPI, true, Operand<TI>::F8>;
     static int max_pairs[64] = {};
     int dev = 0;
     RT(cudaGetDevice(&dev));
@@ -1754,7 +1754,7 @@ struct GemmI8 {
 };
 
 // The kernels of an int8 product: the choice of `kernel` -1, else what the caller asks for.
-enum I8Kernel : int { kI8Single = 0, kI8Pair = 1, kI8Split = 2 };   // kI8Split + S: the split over S CTAs
+enum I8Kernel : int { kI8Pair = 1, kI8Split = 2 };   // kI8Split + S: the split over S CTAs
 
 // Tiles of the split kernel with TN tokens each.
 static long long i8_split_tiles(const GemmI8& p, int TN) { return ((p.N + 127LL) / 128) * ((p.M + TN - 1) / TN); }
@@ -1783,9 +1783,7 @@ static int pick_i8_split(long long tiles, int blocks, int num_sms)
 
 static int pick_i8_kernel(const GemmI8& p, int num_sms)
 {
-    if (i8_split_tiles(p, 64) <= 2 * num_sms) return kI8Split;
-    const long long pairs = ((p.M + 255LL) / 256) * ((p.N + 255) / 256);
-    return pairs >= 2 * num_sms ? kI8Pair : kI8Single;
+    return i8_split_tiles(p, 64) <= 2 * num_sms ? kI8Split : kI8Pair;
 }
 
 template <typename TO, int EPI, int TN>
@@ -1825,6 +1823,37 @@ static void launch_gemm_i8_split(const GemmI8& p, const CUtensorMap& mw, long lo
     RT(cudaLaunchKernelEx(&cfg, gemm_i8_split_kernel<TO, EPI, TN>, ma, mw, out, err));
 }
 
+// As many CTA pairs as can be resident at once, or as there are tiles.
+template <typename TO, int EPI>
+static void launch_gemm_i8_pair(const GemmI8& p, const CUtensorMap& ma, const CUtensorMap& mw, const CUtensorMap& mc,
+                                uint32_t* err, cudaStream_t s)
+{
+    using C = I8PairCfg;
+    static int max_pairs[64] = {};
+    int dev = 0;
+    RT(cudaGetDevice(&dev));
+    if (dev < 0 || dev >= 64) throw std::runtime_error("cudanet_b200: device index out of range");
+    if (!max_pairs[dev]) {
+        RT(cudaFuncSetAttribute(gemm_i8_pair_kernel<TO, EPI>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)C::SMEM));
+        int sms = 0;
+        RT(cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, dev));
+        cudaLaunchConfig_t cfg = {};
+        cfg.gridDim = dim3(static_cast<unsigned>(sms & ~1));
+        cfg.blockDim = dim3(C::THREADS);
+        cfg.dynamicSmemBytes = C::SMEM;
+        int clusters = 0;
+        RT(cudaOccupancyMaxActiveClusters(&clusters, gemm_i8_pair_kernel<TO, EPI>, &cfg));
+        if (clusters < 1) throw std::runtime_error("cudanet_b200: no CTA pair fits on this device");
+        max_pairs[dev] = clusters;
+    }
+    const int n_tiles = (p.N + 255) / 256;
+    const long long tiles = (p.M + 255LL) / 256 * n_tiles;
+    if (tiles > 0x7FFFFFFF) throw std::runtime_error("cudanet_k_gemm_i8: too many tiles");
+    const int pairs = static_cast<int>(std::min<long long>(tiles, max_pairs[dev]));
+    const I8Out out{p.rowscale, p.colscale, p.bias, p.C, p.ldc, p.M, p.N, p.K, n_tiles};
+    launch_k(gemm_i8_pair_kernel<TO, EPI>, dim3(2 * pairs), dim3(C::THREADS), C::SMEM, s, ma, mw, mc, out, err);
+}
+
 template <typename TO, int EPI>
 static void launch_gemm_i8_t(const GemmI8& p, int kernel, cudaStream_t s)
 {
@@ -1839,7 +1868,7 @@ static void launch_gemm_i8_t(const GemmI8& p, int kernel, cudaStream_t s)
     if (!units && kernel < kI8Split) kernel = kI8Split;
     const auto pitch = [](long long ld, int width, int rows) { return rows > 1 ? ld : (width + 15LL) / 16 * 16; };
     const long long pa = pitch(p.lda, p.K, p.M);
-    const CUtensorMap mw = make_map(p.W, MapType::U8, p.K, p.N, pitch(p.ldw, p.K, p.N), 128, kernel == kI8Single ? 256 : 128);
+    const CUtensorMap mw = make_map(p.W, MapType::U8, p.K, p.N, pitch(p.ldw, p.K, p.N), 128, 128);
     if (kernel >= kI8Split) {
         const int split = kernel - kI8Split;
         switch (pick_i8_tokens(p, sms)) {
@@ -1854,10 +1883,8 @@ static void launch_gemm_i8_t(const GemmI8& p, int kernel, cudaStream_t s)
     constexpr MapType t = std::is_same<TO, float>::value    ? MapType::F32
                           : std::is_same<TO, __half>::value ? MapType::F16
                                                             : MapType::BF16;
-    const CUtensorMap mc = make_map(p.C, t, p.N, p.M, pitch(p.ldc, p.N, p.M), 128 / sizeof(TO), 32);
-    const EpiArgs ep{p.bias, p.colscale, 1.f, 0, p.rowscale};
-    if (kernel == kI8Pair) launch_gemm_pair<int8_t, TO, EPI>(ma, mw, mc, p.M, p.N, p.K, ep, err, s);
-    else launch_gemm_bn<int8_t, TO, 256, EPI>(ma, mw, mc, p.M, p.N, p.K, ep, err, sms, s);
+    const CUtensorMap mc = make_map(p.C, t, p.N, p.M, pitch(p.ldc, p.N, p.M), 64 / sizeof(TO), 32, true);
+    launch_gemm_i8_pair<TO, EPI>(p, ma, mw, mc, err, s);
 }
 
 // A null pointer, or one whose address is no multiple of `align`, named in the reason.
@@ -2445,8 +2472,8 @@ CUDANET_API int cudanet_k_gemm_i8(int dtype, int epi, int kernel, const void* A,
         const char* who = "cudanet_k_gemm_i8";
         if (dtype != 0 && dtype != 1) throw std::runtime_error(std::string(who) + ": dtype must be 0 (f16) or 1 (bf16)");
         if (epi < 0 || epi > 3) throw std::runtime_error(std::string(who) + ": epi must be 0..3");
-        if (kernel < -1 || (kernel > 2 && kernel != 3 && kernel != 4 && kernel != 6 && kernel != 10))
-            throw std::runtime_error(std::string(who) + ": kernel must be -1, 0, 1, 2, 3, 4, 6 or 10");
+        if (kernel != -1 && kernel != 1 && kernel != 2 && kernel != 3 && kernel != 4 && kernel != 6 && kernel != 10)
+            throw std::runtime_error(std::string(who) + ": kernel must be -1, 1, 2, 3, 4, 6 or 10");
         if (M < 0 || N < 1 || K < 1 || K > mf::kI8MaxK || M > mf::kI8MaxRows || N > mf::kI8MaxRows)
             throw std::runtime_error(std::string(who) + ": bad sizes (0 <= M, 1 <= N, both <= 2^30, 1 <= K <= 131071)");
         if (M == 0) return 0;

@@ -369,6 +369,29 @@ __device__ __forceinline__ void umma_commit_pair(uint32_t bar_cluster_addr)
                  : "memory");
 }
 
+// Arrive once on the barrier at this shared-memory offset in both CTAs of the pair when the MMAs that this thread
+// issued have completed.
+__device__ __forceinline__ void umma_commit_pair_both(uint64_t* bar)
+{
+    asm volatile(
+        "tcgen05.commit.cta_group::2.mbarrier::arrive::one.shared::cluster.multicast::cluster.b64 [%0], %1;" ::"r"(
+            smem_u32(bar)),
+        "h"(static_cast<uint16_t>(3))
+        : "memory");
+}
+
+// True in one lane of a converged warp, the same one every time.
+__device__ __forceinline__ bool elect_one()
+{
+    uint32_t one;
+    asm volatile(
+        "{\n\t.reg .pred p;\n\t"
+        "elect.sync _|p, 0xffffffff;\n\t"
+        "selp.u32 %0, 1, 0, p;\n\t}"
+        : "=r"(one));
+    return one != 0;
+}
+
 // 32 lanes x 32 columns of 32 bits: thread t of the warp gets lane (base lane + t), columns col..col+31.
 __device__ __forceinline__ void tmem_ld_32x32b_x16(uint32_t taddr, uint32_t (&r)[16])
 {
