@@ -1756,39 +1756,44 @@ struct GemmI8 {
 // The kernels of an int8 product: the choice of `kernel` -1, else what the caller asks for.
 enum I8Kernel : int { kI8Pair = 1, kI8Split = 2 };   // kI8Split + S: the split over S CTAs
 
-// Tiles of the split kernel with TN tokens each.
-static long long i8_split_tiles(const GemmI8& p, int TN) { return ((p.N + 127LL) / 128) * ((p.M + TN - 1) / TN); }
-
-// Tokens a tile of the split kernel: the fewest whose tiles still run all at once (two CTAs an SM), since the epilogue
-// of a tile takes its tokens' time whatever K is (65 x 2,048 x 1,024 with GELU: 4.7 us with 16, 5.0 with 32, 5.5 with 64,
-// 6.4 with 128; 520 x 2,048 x 1,024: 11.2, 6.4, 6.9, 9.1).
-static int pick_i8_tokens(const GemmI8& p, int num_sms)
+// The split kernel's tokens a tile and CTAs a tile, and its time by the model that chooses them (us): a start, then for
+// each round of CTAs (two an SM at once) a CTA's 128-byte blocks of K, its tokens' epilogue and the exchange of a split,
+// then the bytes that all of them load, and the cluster's reads of one another. The constants are a least-squares fit
+// (without negative ones) to 900 timings of M 1..1,040, K 384..8,192 and N 256..8,324 at every TN and S; over those
+// shapes its choice is 2.4% slower than the best one on average. What it weighs: 65 x 2,048 x 1,024 takes 4.4 us with
+// tiles of 16 tokens, 4.8 with 64 and 5.5 with 128; 33 x 8,192 x 4,096 with 64 tokens and K split in 4 8.1 us, with 16
+// and no split 12.8; 16 x 8,192 x 8,192 9.6 us split in 4, 20.2 unsplit.
+struct I8SplitChoice {
+    int tokens, split;
+    double us;
+};
+static I8SplitChoice pick_i8_split(const GemmI8& p, int num_sms)
 {
-    for (int TN : {16, 32, 64})
-        if (i8_split_tiles(p, TN) <= 2 * num_sms) return TN;
-    return 128;
+    const int blocks = (p.K + 127) / 128;
+    I8SplitChoice best{128, 1, 1e30};
+    for (int TN : {16, 32, 64, 128}) {
+        const double tiles = std::ceil(p.N / 128.) * std::ceil(p.M / double(TN)), share = std::min(p.M, TN);
+        for (int S = 1; S <= 8 && S <= blocks; S *= 2) {
+            const double ctas = tiles * S, of_k = (blocks + S - 1) / S, rounds = std::ceil(ctas / (2. * num_sms));
+            const double us = 1.73 + rounds * (0.267 * of_k + 0.0216 * share + (S > 1 ? 0.67 : 0.)) +
+                              0.0141e-6 * 128. * of_k * (128. + share) * ctas + (S > 1 ? 1.53 * ctas / num_sms : 0.);
+            if (us < best.us) best = {TN, S, us};
+        }
+    }
+    return best;
 }
 
-// CTAs that share a tile's K: more while a third of the SMs stay idle and each keeps two 128-byte blocks of K, or while
-// all run at once and each keeps four (16 x 8,192 x 8,192, 64 tiles: 20.2 us alone, 12.8 with 2, 9.6 with 4, 14.9 with 8;
-// 33 x 1,024 x 1,024, 24 tiles: 4.3, 4.4, 3.8, 4.4).
-static int pick_i8_split(long long tiles, int blocks, int num_sms)
+// The pair kernel's time by the same kind of model: 520 x 8,192 x 4,096 (96 tiles, two rounds) 23.9 us and 27.1 split;
+// 1,040 x 4,096 x 8,192 (80 tiles, two rounds) 42.4 and 31.1; 4,160 x 2,048 x 1,024 13.8 and 16.2.
+static double i8_pair_us(const GemmI8& p, int num_sms)
 {
-    int S = 1;
-    while (S < 8 && ((3 * tiles * 2 * S <= 2 * num_sms && blocks >= 4 * S) ||
-                     (tiles * 2 * S <= 2 * num_sms && blocks >= 8 * S)))
-        S *= 2;
-    return S;
-}
-
-static int pick_i8_kernel(const GemmI8& p, int num_sms)
-{
-    return i8_split_tiles(p, 64) <= 2 * num_sms ? kI8Split : kI8Pair;
+    const double rounds = std::ceil(std::ceil(p.M / 256.) * std::ceil(p.N / 256.) / (num_sms / 2));
+    return 4.5 + rounds * (1.8 + 0.28 * ((p.K + 127) / 128));
 }
 
 template <typename TO, int EPI, int TN>
-static void launch_gemm_i8_split(const GemmI8& p, const CUtensorMap& mw, long long pitch_a, int split, int num_sms,
-                                 uint32_t* err, cudaStream_t s)
+static void launch_gemm_i8_split(const GemmI8& p, const CUtensorMap& mw, long long pitch_a, int split, uint32_t* err,
+                                 cudaStream_t s)
 {
     using C = I8SplitCfg<TN>;
     static bool attr[64] = {};
@@ -1801,8 +1806,7 @@ static void launch_gemm_i8_split(const GemmI8& p, const CUtensorMap& mw, long lo
         attr[dev] = true;
     }
     const int n_tiles = (p.N + 127) / 128, blocks = (p.K + 127) / 128;
-    const long long tiles = i8_split_tiles(p, TN);
-    if (split == 0) split = pick_i8_split(tiles, blocks, num_sms);
+    const long long tiles = (long long)n_tiles * ((p.M + TN - 1) / TN);
     while (split > blocks) split /= 2;   // a CTA without a block would have nothing to wait for
     if (tiles * split > (1LL << 31) - 1) throw std::runtime_error("cudanet_k_gemm_i8: too many tiles");
     const CUtensorMap ma = make_map(p.A, MapType::U8, p.K, p.M, pitch_a, 128, TN);
@@ -1864,18 +1868,20 @@ static void launch_gemm_i8_t(const GemmI8& p, int kernel, cudaStream_t s)
     // a TMA store writes whole 16-byte units, the last of a row past its end too: rows must be made of such units
     const bool units = reinterpret_cast<uintptr_t>(p.C) % 16 == 0 && p.N * sizeof(TO) % 16 == 0 &&
                        (p.M == 1 || p.ldc * sizeof(TO) % 16 == 0);
-    if (kernel < 0) kernel = pick_i8_kernel(p, sms);
-    if (!units && kernel < kI8Split) kernel = kI8Split;
+    I8SplitChoice choice{};
+    if (kernel != kI8Pair || !units) choice = pick_i8_split(p, sms);
+    if (kernel < 0) kernel = choice.us <= i8_pair_us(p, sms) ? kI8Split : kI8Pair;
+    if (!units && kernel == kI8Pair) kernel = kI8Split;
     const auto pitch = [](long long ld, int width, int rows) { return rows > 1 ? ld : (width + 15LL) / 16 * 16; };
     const long long pa = pitch(p.lda, p.K, p.M);
     const CUtensorMap mw = make_map(p.W, MapType::U8, p.K, p.N, pitch(p.ldw, p.K, p.N), 128, 128);
     if (kernel >= kI8Split) {
-        const int split = kernel - kI8Split;
-        switch (pick_i8_tokens(p, sms)) {
-            case 16: launch_gemm_i8_split<TO, EPI, 16>(p, mw, pa, split, sms, err, s); break;
-            case 32: launch_gemm_i8_split<TO, EPI, 32>(p, mw, pa, split, sms, err, s); break;
-            case 64: launch_gemm_i8_split<TO, EPI, 64>(p, mw, pa, split, sms, err, s); break;
-            default: launch_gemm_i8_split<TO, EPI, 128>(p, mw, pa, split, sms, err, s);
+        const int split = kernel > kI8Split ? kernel - kI8Split : choice.split;
+        switch (choice.tokens) {
+            case 16: launch_gemm_i8_split<TO, EPI, 16>(p, mw, pa, split, err, s); break;
+            case 32: launch_gemm_i8_split<TO, EPI, 32>(p, mw, pa, split, err, s); break;
+            case 64: launch_gemm_i8_split<TO, EPI, 64>(p, mw, pa, split, err, s); break;
+            default: launch_gemm_i8_split<TO, EPI, 128>(p, mw, pa, split, err, s);
         }
         return;
     }

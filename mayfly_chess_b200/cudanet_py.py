@@ -586,14 +586,16 @@ def k_layernorm_f8(x, g, b, h, n, d, mul, row_stride=1, dll=None):
 
 # ------------------------------------------------------------------------------------------------ int8 operators
 # These calls queue one kernel and return, so what a call costs on the host is most of what a small one costs (the
-# library's part is about 3.5 us, the launch among it). Hence one straight line of checks that reads each attribute
-# once, the torch objects and the default library looked up once a process, and a reason buffer kept by each thread.
-class _I8(threading.local):
+# library's part is about 3.5 us, the launch among it). Hence one straight condition in each that reads every attribute
+# once; where it does not hold, _i8_matrix and _i8_vector find out why, or let the call through (a matrix of one column
+# may have any step). The torch objects and the default library are looked up once a process, the reason buffer is kept
+# by each thread.
+class _I8Reason(threading.local):
     def __init__(self):
-        self.reason = ctypes.create_string_buffer(ERR_LEN)
+        self.buffer = ctypes.create_string_buffer(ERR_LEN)
 
 
-_i8_local = _I8()
+_i8_reason = _I8Reason()
 _i8_once = None
 
 
@@ -627,41 +629,34 @@ def _i8_setup():
     return _i8_once
 
 
-def _i8_bad_type(name, t, want):
-    return ValueError(f"{name}: {want} only, got {t.dtype}")
+def _i8_type(once, t, name):
+    """The C ABI's code of a tensor's element type: 0 f16, 1 bf16, 2 f32."""
+    code = once.types.get(t.dtype)
+    if code is None:
+        raise ValueError(f"{name}: float16, bfloat16 or float32 only, got {t.dtype}")
+    return code
 
 
-def _i8_rows(t, name, shape, dev):
-    """The row pitch of a matrix of this shape on device index dev, its rows contiguous."""
-    if t.shape != shape:
-        raise ValueError(f"{name}: shape {tuple(t.shape)}, expected {tuple(shape)}")
-    if t.get_device() != dev or dev < 0:
+def _i8_matrix(t, name, shape, dev, dtype=None):
+    """Raises unless t is a matrix of this shape and dtype (None: any) on device index dev with contiguous rows."""
+    if dtype is not None and t.dtype is not dtype:
+        raise ValueError(f"{name}: {dtype} only, got {t.dtype}")
+    if len(t.shape) != 2 or t.shape != shape:
+        raise ValueError(f"{name}: shape {tuple(t.shape)}, expected {tuple(shape) if len(shape) == 2 else 'a matrix'}")
+    if dev < 0 or t.get_device() != dev:
         raise ValueError(f"{name}: on {t.device}, expected a tensor of one CUDA device with the others")
-    pitch, step = t.stride()
-    if step != 1 and shape[1] > 1:
+    if t.stride(1) != 1 and shape[1] > 1:
         raise ValueError(f"{name}: rows must be contiguous, got strides {t.stride()}")
-    return pitch
 
 
-def _i8_vec(t, name, n, dev, f32):
-    """The address of a contiguous float32 vector of n elements on device index dev."""
-    if t.dtype is not f32:
-        raise _i8_bad_type(name, t, "float32")
+def _i8_vector(once, t, name, n, dev):
+    """Raises unless t is a contiguous float32 vector of n elements on device index dev."""
+    if t.dtype is not once.f32:
+        raise ValueError(f"{name}: float32 only, got {t.dtype}")
     if t.shape != (n,) or not t.is_contiguous():
         raise ValueError(f"{name}: shape {tuple(t.shape)} strides {t.stride()}, expected ({n},) contiguous")
     if t.get_device() != dev:
         raise ValueError(f"{name}: on {t.device}, expected a tensor of one CUDA device with the others")
-    return t.data_ptr()
-
-
-def _i8_call(once, fn, dev, *args):
-    """fn(*args, stream, reason) on device `dev` and its current stream; RuntimeError with the library's reason."""
-    if once.device() != dev:
-        with once.on_device(dev):
-            return _i8_call(once, fn, dev, *args)
-    reason = _i8_local.reason
-    if fn(*args, once.stream(dev), reason, ERR_LEN) != 0:
-        raise RuntimeError(f"{fn.__name__}: {_msg(reason)}")
 
 
 def k_rmsnorm_i8(x, delta, g, out, q, scale, eps=1e-6, dll=None):
@@ -671,33 +666,38 @@ def k_rmsnorm_i8(x, delta, g, out, q, scale, eps=1e-6, dll=None):
     int8, scale (M,) float32. Rows may have any pitch; asynchronous on the device's current stream. Returns (q,
     scale)."""
     once = _i8_once or _i8_setup()
-    xt = once.types.get(x.dtype)
-    if xt is None:
-        raise _i8_bad_type("x", x, "float16, bfloat16 or float32")
-    if q.dtype is not once.int8:
-        raise _i8_bad_type("q", q, "int8")
-    shape, dev = x.shape, x.get_device()
-    if len(shape) != 2:
-        raise ValueError(f"x: shape {tuple(shape)}, expected a matrix")
-    M, D = shape
-    ldx, ldq = _i8_rows(x, "x", shape, dev), _i8_rows(q, "q", shape, dev)
+    f32, shape, dev, xt = once.f32, x.shape, x.get_device(), _i8_type(once, x, "x")
+    xs, qs = x.stride(), q.stride()
+    if (len(shape) != 2 or dev < 0 or xs[1] != 1 or q.dtype is not once.int8 or q.shape != shape or qs[1] != 1
+            or q.get_device() != dev or g.dtype is not f32 or g.shape != shape[1:] or g.get_device() != dev
+            or not g.is_contiguous() or scale.dtype is not f32 or scale.shape != shape[:1]
+            or scale.get_device() != dev or not scale.is_contiguous()):
+        _i8_matrix(x, "x", shape, dev)
+        _i8_matrix(q, "q", shape, dev, once.int8)
+        _i8_vector(once, g, "g", shape[1], dev)
+        _i8_vector(once, scale, "scale", shape[0], dev)
     if delta is None:
         if out is not None:
             raise ValueError("out without delta: there is no sum to store")
         dt, ldd, ldo, dp, op = xt, 0, 0, None, None
     else:
-        dt = once.types.get(delta.dtype)
-        if dt is None:
-            raise _i8_bad_type("delta", delta, "float16, bfloat16 or float32")
+        dt = _i8_type(once, delta, "delta")
         if out is None:
             raise ValueError("delta without out: out holds the sum (x itself: in place)")
-        if out.dtype is not x.dtype:
-            raise _i8_bad_type("out", out, f"x's {x.dtype}")
-        ldd, ldo = _i8_rows(delta, "delta", shape, dev), ldx if out is x else _i8_rows(out, "out", shape, dev)
-        dp, op = delta.data_ptr(), out.data_ptr()
-    _i8_call(once, once.load(dll).cudanet_k_rmsnorm_i8, dev, xt, dt, x.data_ptr(), dp,
-             _i8_vec(g, "g", D, dev, once.f32), op, q.data_ptr(), _i8_vec(scale, "scale", M, dev, once.f32), M, D, ldx,
-             ldd, ldo, ldq, eps)
+        ds, os_ = delta.stride(), out.stride()
+        if (delta.shape != shape or delta.get_device() != dev or ds[1] != 1 or out.dtype is not x.dtype
+                or out.shape != shape or out.get_device() != dev or os_[1] != 1):
+            _i8_matrix(delta, "delta", shape, dev)
+            _i8_matrix(out, "out", shape, dev, x.dtype)
+        ldd, ldo, dp, op = ds[0], os_[0], delta.data_ptr(), out.data_ptr()
+    if once.device() != dev:
+        with once.on_device(dev):
+            return k_rmsnorm_i8(x, delta, g, out, q, scale, eps, dll)
+    reason = _i8_reason.buffer
+    if (once.lib if dll is None and once.lib else once.load(dll)).cudanet_k_rmsnorm_i8(
+            xt, dt, x.data_ptr(), dp, g.data_ptr(), op, q.data_ptr(), scale.data_ptr(), shape[0], shape[1], xs[0], ldd,
+            ldo, qs[0], eps, once.stream(dev), reason, ERR_LEN) != 0:
+        raise RuntimeError(f"cudanet_k_rmsnorm_i8: {_msg(reason)}")
     return q, scale
 
 
@@ -706,18 +706,22 @@ def k_quant_i8(x, q, scale, dll=None):
     stands for x. A weight matrix (N, K) gets a scale for each output channel. Rows may have any pitch; asynchronous on
     the device's current stream. Returns (q, scale)."""
     once = _i8_once or _i8_setup()
-    xt = once.types.get(x.dtype)
-    if xt is None:
-        raise _i8_bad_type("x", x, "float16, bfloat16 or float32")
-    if q.dtype is not once.int8:
-        raise _i8_bad_type("q", q, "int8")
-    shape, dev = x.shape, x.get_device()
-    if len(shape) != 2:
-        raise ValueError(f"x: shape {tuple(shape)}, expected a matrix")
-    M, D = shape
-    ldx, ldq = _i8_rows(x, "x", shape, dev), _i8_rows(q, "q", shape, dev)
-    _i8_call(once, once.load(dll).cudanet_k_quant_i8, dev, xt, x.data_ptr(), q.data_ptr(),
-             _i8_vec(scale, "scale", M, dev, once.f32), M, D, ldx, ldq)
+    shape, dev, xt = x.shape, x.get_device(), _i8_type(once, x, "x")
+    xs, qs = x.stride(), q.stride()
+    if (len(shape) != 2 or dev < 0 or xs[1] != 1 or q.dtype is not once.int8 or q.shape != shape or qs[1] != 1
+            or q.get_device() != dev or scale.dtype is not once.f32 or scale.shape != shape[:1]
+            or scale.get_device() != dev or not scale.is_contiguous()):
+        _i8_matrix(x, "x", shape, dev)
+        _i8_matrix(q, "q", shape, dev, once.int8)
+        _i8_vector(once, scale, "scale", shape[0], dev)
+    if once.device() != dev:
+        with once.on_device(dev):
+            return k_quant_i8(x, q, scale, dll)
+    reason = _i8_reason.buffer
+    if (once.lib if dll is None and once.lib else once.load(dll)).cudanet_k_quant_i8(
+            xt, x.data_ptr(), q.data_ptr(), scale.data_ptr(), shape[0], shape[1], xs[0], qs[0], once.stream(dev),
+            reason, ERR_LEN) != 0:
+        raise RuntimeError(f"cudanet_k_quant_i8: {_msg(reason)}")
     return q, scale
 
 
@@ -726,22 +730,37 @@ def k_gemm_i8(A, W, rowscale, colscale, bias, C, epi, kernel=-1, dll=None):
     16 bytes, the sum exact in int32, rowscale (M,), colscale (N,) and bias (N,) or None float32: epi 0 16-bit out, 1
     GELU and 16-bit out, 2 C += (float32), 3 float32 out. Asynchronous on the device's current stream. Returns C."""
     once = _i8_once or _i8_setup()
-    if A.dtype is not once.int8:
-        raise _i8_bad_type("A", A, "int8")
-    if W.dtype is not once.int8:
-        raise _i8_bad_type("W", W, "int8")
-    ct = once.types.get(C.dtype)
-    if ct is None or (ct == 2) != (epi >= 2):
-        raise _i8_bad_type("C", C, f"epi {epi} writes float32: it" if epi >= 2 else "float16 or bfloat16")
-    sa, sw, dev = A.shape, W.shape, A.get_device()
+    i8, f32, sa, sw, dev, ct = once.int8, once.f32, A.shape, W.shape, A.get_device(), _i8_type(once, C, "C")
+    if (ct == 2) != (epi >= 2):
+        raise ValueError(f"C: epi {epi} writes {'float32' if epi >= 2 else 'float16 or bfloat16'}, got {C.dtype}")
     if len(sa) != 2 or len(sw) != 2 or sa[1] != sw[1]:
         raise ValueError(f"A and W: shapes {tuple(sa)} and {tuple(sw)}, expected (M, K) and (N, K)")
     M, K = sa
     N = sw[0]
-    lda, ldw, ldc = _i8_rows(A, "A", sa, dev), _i8_rows(W, "W", sw, dev), _i8_rows(C, "C", (M, N), dev)
-    _i8_call(once, once.load(dll).cudanet_k_gemm_i8, dev, ct & 1, epi, kernel, A.data_ptr(), W.data_ptr(),
-             _i8_vec(rowscale, "rowscale", M, dev, once.f32), _i8_vec(colscale, "colscale", N, dev, once.f32),
-             None if bias is None else _i8_vec(bias, "bias", N, dev, once.f32), C.data_ptr(), M, N, K, lda, ldw, ldc)
+    ta, tw, tc = A.stride(), W.stride(), C.stride()
+    if (dev < 0 or A.dtype is not i8 or ta[1] != 1 or W.dtype is not i8 or tw[1] != 1 or W.get_device() != dev
+            or C.shape != (M, N) or tc[1] != 1 or C.get_device() != dev or rowscale.dtype is not f32
+            or rowscale.shape != sa[:1] or rowscale.get_device() != dev or not rowscale.is_contiguous()
+            or colscale.dtype is not f32 or colscale.shape != sw[:1] or colscale.get_device() != dev
+            or not colscale.is_contiguous()):
+        _i8_matrix(A, "A", sa, dev, i8)
+        _i8_matrix(W, "W", sw, dev, i8)
+        _i8_matrix(C, "C", (M, N), dev)
+        _i8_vector(once, rowscale, "rowscale", M, dev)
+        _i8_vector(once, colscale, "colscale", N, dev)
+    bp = None
+    if bias is not None:
+        if (bias.dtype is not f32 or bias.shape != sw[:1] or bias.get_device() != dev or not bias.is_contiguous()):
+            _i8_vector(once, bias, "bias", N, dev)
+        bp = bias.data_ptr()
+    if once.device() != dev:
+        with once.on_device(dev):
+            return k_gemm_i8(A, W, rowscale, colscale, bias, C, epi, kernel, dll)
+    reason = _i8_reason.buffer
+    if (once.lib if dll is None and once.lib else once.load(dll)).cudanet_k_gemm_i8(
+            ct & 1, epi, kernel, A.data_ptr(), W.data_ptr(), rowscale.data_ptr(), colscale.data_ptr(), bp,
+            C.data_ptr(), M, N, K, ta[0], tw[0], tc[0], once.stream(dev), reason, ERR_LEN) != 0:
+        raise RuntimeError(f"cudanet_k_gemm_i8: {_msg(reason)}")
     return C
 
 
