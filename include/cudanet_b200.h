@@ -205,7 +205,8 @@ CUDANET_API int cudanet_k_layernorm_f8(int x_dtype, const void* x, const float* 
  * Device pointers on the current device, queued on `stream` (NULL: the legacy default stream), asynchronous: the call
  * does not wait, allocates nothing and may be captured into a CUDA graph. Types: 0 = f16, 1 = bf16, 2 = f32. Rows have
  * a pitch in elements (not used with a single row); what lies between a row's end and its pitch is neither read into
- * a result nor written. M = 0 does nothing. Return 0, or -1 with the reason in err.
+ * a result nor written. M = 0 does nothing; M <= 2^30. Outputs overlap no other argument, save where it is said. A
+ * process' first call of each kind loads its kernel. Return 0, or -1 with the reason in err.
  *
  * A row's codes are q[i] = rint(t[i] * (127 / a)) (ties to even), a = max |t[i]|, so that -127 <= q <= 127. A row
  * with a < 2^-120 has scale 0 and codes 0. A row that holds a NaN or an infinity (for the norm: or whose sum of
@@ -227,9 +228,11 @@ CUDANET_API int cudanet_k_quant_i8(int x_type, const void* x, void* q, float* sc
  * int32 sum (any int8 codes, -128 included; 1 <= K <= 131,071, the largest K whose sums fit), with epi as for
  * cudanet_k_gemm: 0: C 16-bit (`dtype`) = v; 1: C 16-bit = gelu(v); 2: C f32 += v; 3: C f32 = v. A and W begin on 16
  * bytes and their row pitches are multiples of 16; C, bias and the scales may begin anywhere and C have any pitch
- * >= N. kernel -1 chooses; 0 asks for single-CTA 128 x 256 tiles, 1 for CTA-pair 256 x 256 tiles. Every kernel gives the
- * same bits. M and N up to 2^30. A wait inside the kernel that runs out (a failure of the device) ends it with C
- * unwritten and is reported by cudanet_k_i8_check. */
+ * >= N. kernel -1 chooses; 1 asks for 256 x 256 tiles on CTA pairs (where C's
+ * start, row and pitch are whole 16-byte units, else as 2), 2 for the kernel with weights on the tensor cores' lanes
+ * and K split as it chooses, 3, 4, 6 and 10 for that with K split over 1, 2, 4 and 8 CTAs (fewer where K has fewer
+ * blocks of 128). Every kernel gives the same bits. M and N up to 2^30. A wait inside the kernel that runs out (a failure of the device) ends it with C
+ * partly unwritten and is reported by cudanet_k_i8_check. */
 CUDANET_API int cudanet_k_gemm_i8(int dtype, int epi, int kernel, const void* A, const void* W, const float* rowscale,
                                   const float* colscale, const float* bias, void* C, int M, int N, int K, int64_t lda,
                                   int64_t ldw, int64_t ldc, void* stream, char* err, int err_len);

@@ -1653,7 +1653,7 @@ static void attention_once(const void* qkv, void* att, int B, int d, int heads, 
 // The element types of the int8 entry points: the codes of the 16-bit kernels, and 2 = f32.
 enum I8Type : int { kI8F16 = 0, kI8BF16 = 1, kI8F32 = 2 };
 constexpr int kI8MaxRow = 32768;    // the longest row of the norm and the quantiser
-constexpr int kI8MaxRows = 1 << 30; // rows of A and of W: tile counts and rounded-up sizes stay within int
+constexpr int kI8MaxRows = 1 << 30; // rows of any operand: tile counts and rounded-up sizes stay within int
 constexpr int kI8MaxK = 131071;     // 131,071 products of -128 * -128 are the most that an int32 sum holds
 
 // The word that the int8 products' bounded waits report in, one on every GPU that loads the library: 0, or the first
@@ -2421,8 +2421,8 @@ CUDANET_API int cudanet_k_rmsnorm_i8(int x_type, int delta_type, const void* x, 
             throw std::runtime_error(std::string(who) + ": a type must be 0 (f16), 1 (bf16) or 2 (f32)");
         if (delta && x_type != mf::kI8F32 && delta_type != x_type)
             throw std::runtime_error(std::string(who) + ": delta must be of x's type, or x f32");
-        if (M < 0 || D < 1 || D > mf::kI8MaxRow)
-            throw std::runtime_error(std::string(who) + ": bad sizes (rows >= 0, 1 <= D <= 32768)");
+        if (M < 0 || M > mf::kI8MaxRows || D < 1 || D > mf::kI8MaxRow)
+            throw std::runtime_error(std::string(who) + ": bad sizes (0 <= M <= 2^30, 1 <= D <= 32768)");
         if (!(eps > 0.f) || !std::isfinite(eps)) throw std::runtime_error(std::string(who) + ": eps must be positive");
         if (M == 0) return 0;
         const uintptr_t xb = static_cast<uintptr_t>(mf::i8_bytes(x_type));
@@ -2454,8 +2454,8 @@ CUDANET_API int cudanet_k_quant_i8(int x_type, const void* x, void* q, float* sc
         const char* who = "cudanet_k_quant_i8";
         if (x_type < mf::kI8F16 || x_type > mf::kI8F32)
             throw std::runtime_error(std::string(who) + ": x_type must be 0 (f16), 1 (bf16) or 2 (f32)");
-        if (M < 0 || D < 1 || D > mf::kI8MaxRow)
-            throw std::runtime_error(std::string(who) + ": bad sizes (rows >= 0, 1 <= D <= 32768)");
+        if (M < 0 || M > mf::kI8MaxRows || D < 1 || D > mf::kI8MaxRow)
+            throw std::runtime_error(std::string(who) + ": bad sizes (0 <= M <= 2^30, 1 <= D <= 32768)");
         if (M == 0) return 0;
         mf::need_ptr(who, "x", x, static_cast<uintptr_t>(mf::i8_bytes(x_type)));
         mf::need_ptr(who, "q", q, 1);

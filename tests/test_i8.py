@@ -46,7 +46,7 @@ NORM = ("x_type", "delta_type", "x", "delta", "g", "out", "q", "scale", "M", "D"
 
 @pytest.mark.parametrize("reason,change", [
     ("type", {"x_type": 3}), ("type", {"delta_type": -1}), ("x's type", {"x_type": 1, "delta_type": 0}),
-    ("x's type", {"x_type": 0, "delta_type": 2}), ("bad sizes", {"M": -3}), ("bad sizes", {"D": 0}),
+    ("x's type", {"x_type": 0, "delta_type": 2}), ("bad sizes", {"M": -3}), ("bad sizes", {"M": 2 ** 30 + 1}), ("bad sizes", {"D": 0}),
     ("bad sizes", {"D": 32769}), ("eps", {"eps": 0.0}), ("eps", {"eps": float("nan")}), ("eps", {"eps": float("inf")}),
     ("x is a null", {"x": None}), ("g is a null", {"g": None}), ("q is a null", {"q": None}),
     ("scale is a null", {"scale": None}), ("out is a null", {"out": None}), ("out without delta", {"delta": None}),

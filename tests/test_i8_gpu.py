@@ -37,18 +37,18 @@ def gen(seed):
 
 
 def matrix(rows, cols, dtype, pitch=None, fill=0, offset=0):
-    """A (rows, cols) view, `offset` elements into a buffer of rows of `pitch` that is filled with `fill`; and the
-    buffer."""
+    """A (rows, cols) view, `offset` elements into a buffer of rows of `pitch` that is filled with `fill`, two rows more
+    than the view's; and the buffer."""
     pitch = cols if pitch is None else pitch
-    full = torch.full((rows * pitch + offset,), fill, dtype=dtype, device="cuda")
-    return full[offset:].view(rows, pitch)[:, :cols], full
+    full = torch.full(((rows + 2) * pitch + offset,), fill, dtype=dtype, device="cuda")
+    return full[offset:].view(rows + 2, pitch)[:rows, :cols], full
 
 
 def untouched(view, full, fill, offset=0):
     """Whether nothing outside the view was written."""
     keep = full.clone()
     rows, cols = view.shape
-    keep[offset:].view(rows, -1)[:, :cols] = fill
+    keep[offset:].view(rows + 2, -1)[:rows, :cols] = fill
     want = torch.full_like(full, fill)
     return torch.equal(keep.view(torch.uint8), want.view(torch.uint8))
 
@@ -393,6 +393,36 @@ def test_block_on_another_stream_and_replayed(k):
         for b in blocks:
             assert all(torch.equal(b[n], t) for n, t in zip(("out", "q", "q2", "h"), want[1]))
     del graphs
+
+
+def test_first_call_of_a_process_captured(k):
+    """Each operator's first call of a process inside a stream capture: nothing in it may need an earlier call."""
+    import subprocess
+    import sys
+
+    from conftest import REPO
+    code = """
+import torch
+from mayfly_chess_b200 import cudanet_py as k
+M, K, N = 300, 256, 512
+e = lambda *n, dtype=torch.float32: torch.zeros(*n, dtype=dtype, device="cuda")
+x, q, s, w, c = torch.ones(M, K, device="cuda"), e(M, K, dtype=torch.int8), e(M), e(N, K, dtype=torch.int8), e(N)
+C, B = e(M, N), torch.full((N, K), 2.0, device="cuda")
+torch.cuda.synchronize()
+g = torch.cuda.CUDAGraph()
+with torch.cuda.graph(g):
+    k.k_quant_i8(B, w, c)
+    k.k_rmsnorm_i8(x, x, torch.ones_like(c[:K]), x, q, s)
+    for kernel in (-1, 1, 10):
+        k.k_gemm_i8(q, w, s, c, None, C, 2, kernel)
+g.replay()
+torch.cuda.synchronize()
+k.k_i8_check()
+# out = 2 in place, its norm 1, times a weight of 2: K * 2 for each of the three products added
+assert (x == 2).all() and ((C / (3 * 2 * K) - 1).abs() < 1e-5).all(), C
+"""
+    r = subprocess.run([sys.executable, "-c", code], cwd=REPO, capture_output=True, text=True, timeout=300)
+    assert r.returncode == 0, r.stderr[-2000:]
 
 
 def test_no_rows(k):
