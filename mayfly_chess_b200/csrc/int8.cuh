@@ -107,7 +107,8 @@ __device__ __forceinline__ uint32_t codes4(float a, float b, float c, float d, f
 }
 
 // L threads hold a row in registers (8, 16 or 32 of a warp, or a block, L = 0), 8 V elements a thread, so x and delta
-// are read and out, q and scale written once: bound by HBM from about a thousand rows. VEC: neighbouring elements 8 at a
+// are read and out, q and scale written once: bound by HBM from about a thousand rows (norm 66,560 x 1,024, f32 + bf16:
+// 110 us, 6.8 TB/s; quantiser 66,560 x 2,048 bf16: 59 us, 6.9 TB/s). VEC: neighbouring elements 8 at a
 // time (D a multiple of 8, every row of every operand begins on 16 bytes, q's on 8); else element by element.
 template <typename XT, typename DT, bool NORM, bool VEC, int L, int V>
 __global__ void __launch_bounds__(L ? 256 : 1024) rows_i8_kernel(const RowsI8 a)
@@ -294,11 +295,15 @@ struct I8Out {
 // ------------------------------------------------------------------------------------------------ many rows
 // 256 x 256 tiles on CTA pairs (tcgen05.mma.cta_group::2, kind::i8), persistent: each CTA holds 128 rows of A, 128 of the
 // 256 rows of W and 128 x 256 accumulators, two of them, so that a tile's epilogue runs under the next tile's products.
-// What bounds it is shared memory's bandwidth: at the full rate of the products the operands' arrival takes half of the
-// 128 bytes a cycle and their reading the other half, and the epilogue's staging comes on top. So a pair takes
-// neighbouring tiles, W's blocks fastest, and keeps its rows of A in shared memory over all of them where they fit
-// (K <= 1,024): only W then streams. Roles: warp 0 TMA loads, warp 1 tensor memory and the products (leader CTA),
-// warps 2..17 the epilogue.
+// At the full rate of the products the operands' arrival takes half of shared memory's 128 bytes a cycle and their
+// reading the other half, and the epilogue's staging comes on top. So a pair takes neighbouring tiles, W's blocks
+// fastest, and keeps its rows of A in shared memory over all of them where they fit (K <= 1,024): only W then streams.
+// What paced the products before was their issue: by one lane of a diverged warp, with two commits a stage, 187 cycles an
+// instruction; from a converged warp with one commit to both CTAs 128 to 140 (66,560 x 2,048 x 1,024: 131 -> 113 us).
+// What bounds it now: 8,192^3 keeps the tensor cores busy 92% of their cycles (2,630 TOP/s); the 1,000 W cap, which takes
+// the clock from 1.97 to about 1.4 GHz in a long run (66,560 x 2,048 x 1,024 there 134 us, with GELU 147); and with GELU
+// the epilogue's instructions (7,100 cycles a tile against 6,100 without it and 4,096 of products). Roles: warp 0 TMA
+// loads, warp 1 tensor memory and the products (leader CTA), warps 2..17 the epilogue.
 struct I8PairCfg {
     static constexpr int SLOTS = 11;                     // of 128 rows x 128 bytes
     static constexpr uint32_t SLOT = 128 * 128;
@@ -579,7 +584,9 @@ gemm_i8_pair_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_consta
 // waste little and a thread of the epilogue owns an output channel: its column scale and bias stay in two registers,
 // and a warp stores 32 neighbouring channels of a row, wherever the row begins. K is split over a cluster of S CTAs,
 // which fills the GPU where the tiles alone do not: each CTA leaves its exact int32 partial sums in its shared memory
-// and sums a share of the tokens over the cluster through distributed shared memory. No workspace, no atomics.
+// and sums a share of the tokens over the cluster through distributed shared memory. No workspace, no atomics. Bound by
+// what W takes from HBM plus about 5 us (start, first bytes, exchange): 16 x 32,768 x 8,192 45.6 us (5.9 TB/s), 16 x 8,192
+// x 8,192 15.2 us, out of L2 9.4 us; 1 x 8,324 x 1,024 4.3 us; 66,560 x 2,047 x 1,024 (rows that TMA cannot store) 230 us.
 template <int TN> struct I8SplitCfg {
     static constexpr uint32_t W_BYTES = 128 * 128, A_BYTES = TN * 128, STAGE_BYTES = W_BYTES + A_BYTES;
     static constexpr int STAGES = TN == 128 ? 3 : TN == 64 ? 4 : 5;   // two CTAs an SM

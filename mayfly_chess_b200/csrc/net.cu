@@ -1692,7 +1692,7 @@ static void launch_rows_i8_cfg(const RowsI8& a, int num_sms, cudaStream_t s)
 
 // Part of a warp up to 1,024 elements (2,048 for the 16-bit quantiser), then a block a row: as few threads as hold the
 // row with enough loads on their way. Measured (GB/s, 66,560 x 2,048 bf16 quantised: a warp of 8 vectors a thread 6,946,
-// a block of 4 5,843; 4,097 x 8,192 bf16 norm: blocks of 4 vectors 6,138, of 2 5,312, of 1 4,327). Rows that are read
+// a block of 2 5,843; 4,097 x 8,192 bf16 norm: blocks of 4 vectors 6,138, of 2 5,312, of 1 4,327). Rows that are read
 // element by element: 20,871 x 727 f16 quantised in a warp 2,829, in a block 1,978; 16,000 x 4,001 f16 norm in blocks of
 // 8 elements a thread 2,285, of 16 1,619, of 32 1,488, the quantiser there 1,822, 2,327 and 1,960.
 template <typename XT, typename DT, bool NORM>
