@@ -127,7 +127,7 @@ static CUtensorMap operand_map(const void* base, MapType type, uint64_t K, uint6
 // boxes of one epilogue store (GemmCfg::ROW_BYTES wide: 64-byte rows for the GELU epilogues, the bf16 residual
 // and the bias epilogue of an FP8 product, `f8`; store_rows(epi, f8) rows high). The residuals' maps take TMA
 // reduce-adds into X.
-static CUtensorMap output_map(void* base, int epi, MapType t16, int M, int N, long long ldc, bool f8 = false)
+static CUtensorMap output_map(void* base, int epi, MapType t16, int M, int N, int ldc, bool f8 = false)
 {
     const uint32_t rows = static_cast<uint32_t>(store_rows(epi, f8));
     if (epi == kEpiResidual || epi == kEpiF32) return make_map(base, MapType::F32, N, M, ldc, 32, rows);

@@ -13,7 +13,8 @@ logits at each row's legal moves, 0 on padding), val (B,) and qv (B, wide).
 
 Additions: evaluate_logits (also the full (B, 8324) logits), begin/end (two batches in flight),
 evaluate_device (torch CUDA tensors in and out, queued on a stream), precision, check, calibrate (the input
-ranges an e4m3 weight file's static scales come from), and k_* single-kernel entry points for unit tests.
+ranges an e4m3 weight file's static scales come from), k_* single-kernel entry points for unit tests, and the int8
+linear layer with dynamic scales (k_rmsnorm_i8, k_quant_i8, k_gemm_i8, k_i8_check; asynchronous on the current stream).
 
 The library is MAYFLY_CUDANET_DLL, else libcudanet_b200.so beside this file. There is no fallback: if the
 library is missing the constructor raises.
