@@ -121,13 +121,18 @@ __global__ void __launch_bounds__(L ? 256 : 1024) rows_i8_kernel(const RowsI8 a)
     // a warp that holds a row at all goes on as a whole, its threads without one with no elements
     if (L && row - (threadIdx.x & 31) / (L ? L : 1) >= (size_t)a.M) return;
     const int D = row < (size_t)a.M ? a.D : 0;
-    const XT* __restrict__ x = static_cast<const XT*>(a.x) + row * a.ldx;
-    const DT* __restrict__ delta = static_cast<const DT*>(a.delta) + row * a.ldd;
-    XT* out = static_cast<XT*>(a.out) + row * a.ldo;
-    int8_t* q = a.q + row * a.ldq;
+    // This thread's first element, and the elements from there to the row's end: element j of vector v lies at(v, j)
+    // further on. Element by element a warp has 256 V neighbours, so that the distances are constants: what such a row
+    // costs is instructions.
+    const int e0 = VEC ? 8 * t : L ? t : (t >> 5) * 256 * V + (t & 31);
+    const int left = D - e0;
+    auto at = [&](int v, int j) { return VEC ? 8 * T * v + j : 256 * v + 32 * j; };
+    const XT* __restrict__ x = static_cast<const XT*>(a.x) + row * a.ldx + e0;
+    const DT* __restrict__ delta = static_cast<const DT*>(a.delta) + row * a.ldd + e0;
+    const float* __restrict__ gp = NORM ? a.g + e0 : nullptr;
+    XT* out = static_cast<XT*>(a.out) + row * a.ldo + e0;
+    int8_t* q = a.q + row * a.ldq + e0;
     const bool add = NORM && a.delta;
-    // element j of vector v of this thread
-    auto at = [&](int v, int j) { return VEC ? 8 * (t + T * v) + j : t + T * (8 * v + j); };
 
     float s[V][8], d[V][8];
     if constexpr (VEC) {
@@ -136,13 +141,13 @@ __global__ void __launch_bounds__(L ? 256 : 1024) rows_i8_kernel(const RowsI8 a)
 #pragma unroll
         for (int v = 0; v < V; ++v) {
             rx[v].zero();
-            if (at(v, 0) < D) rx[v].load(x + at(v, 0));
+            if (at(v, 0) < left) rx[v].load(x + at(v, 0));
         }
         if (add) {
 #pragma unroll
             for (int v = 0; v < V; ++v) {
                 rd[v].zero();
-                if (at(v, 0) < D) rd[v].load(delta + at(v, 0));
+                if (at(v, 0) < left) rd[v].load(delta + at(v, 0));
             }
         }
 #pragma unroll
@@ -156,13 +161,13 @@ __global__ void __launch_bounds__(L ? 256 : 1024) rows_i8_kernel(const RowsI8 a)
 #pragma unroll
         for (int v = 0; v < V; ++v) {
 #pragma unroll
-            for (int j = 0; j < 8; ++j) rx[v][j] = at(v, j) < D ? x[at(v, j)] : from_f32<XT>(0.f);
+            for (int j = 0; j < 8; ++j) rx[v][j] = at(v, j) < left ? x[at(v, j)] : from_f32<XT>(0.f);
         }
         if (add) {
 #pragma unroll
             for (int v = 0; v < V; ++v) {
 #pragma unroll
-                for (int j = 0; j < 8; ++j) rd[v][j] = at(v, j) < D ? delta[at(v, j)] : from_f32<DT>(0.f);
+                for (int j = 0; j < 8; ++j) rd[v][j] = at(v, j) < left ? delta[at(v, j)] : from_f32<DT>(0.f);
             }
         }
 #pragma unroll
@@ -180,11 +185,11 @@ __global__ void __launch_bounds__(L ? 256 : 1024) rows_i8_kernel(const RowsI8 a)
 #pragma unroll
             for (int j = 0; j < 8; ++j) s[v][j] = to_f32(from_f32<XT>(s[v][j] + d[v][j]));
             if constexpr (VEC) {
-                if (at(v, 0) < D) store8(out + at(v, 0), s[v]);
+                if (at(v, 0) < left) store8(out + at(v, 0), s[v]);
             } else {
 #pragma unroll
                 for (int j = 0; j < 8; ++j)
-                    if (at(v, j) < D) out[at(v, j)] = from_f32<XT>(s[v][j]);
+                    if (at(v, j) < left) out[at(v, j)] = from_f32<XT>(s[v][j]);
             }
         }
     }
@@ -197,11 +202,11 @@ __global__ void __launch_bounds__(L ? 256 : 1024) rows_i8_kernel(const RowsI8 a)
             if constexpr (VEC) {
                 Raw8<float> rg;
                 rg.zero();
-                if (at(v, 0) < D) rg.load(a.g + at(v, 0));
+                if (at(v, 0) < left) rg.load(gp + at(v, 0));
                 rg.get(g);
             } else {
 #pragma unroll
-                for (int j = 0; j < 8; ++j) g[j] = at(v, j) < D ? __ldg(a.g + at(v, j)) : 0.f;
+                for (int j = 0; j < 8; ++j) g[j] = at(v, j) < left ? __ldg(gp + at(v, j)) : 0.f;
             }
 #pragma unroll
             for (int j = 0; j < 8; ++j) {
@@ -239,17 +244,22 @@ __global__ void __launch_bounds__(L ? 256 : 1024) rows_i8_kernel(const RowsI8 a)
     }
     const RowScale rs = row_scale(mx, NORM ? rsqrtf(ss / static_cast<float>(a.D) + a.eps) : 1.f);
     if (t == 0 && D) a.scale[row] = rs.scale;
-    const uint32_t live = rs.inv == 0.f ? 0u : 0xFFFFFFFFu;   // a row without a scale has codes 0, whatever it holds
+    if (rs.inv == 0.f) {   // a row without a scale has codes 0, whatever it holds
+#pragma unroll
+        for (int v = 0; v < V; ++v)
+#pragma unroll
+            for (int j = 0; j < 8; ++j) s[v][j] = 0.f;
+    }
 #pragma unroll
     for (int v = 0; v < V; ++v) {
-        const uint32_t lo = codes4(s[v][0], s[v][1], s[v][2], s[v][3], rs.inv) & live;
-        const uint32_t hi = codes4(s[v][4], s[v][5], s[v][6], s[v][7], rs.inv) & live;
         if constexpr (VEC) {
-            if (at(v, 0) < D) *reinterpret_cast<uint2*>(q + at(v, 0)) = make_uint2(lo, hi);
+            if (at(v, 0) < left)
+                *reinterpret_cast<uint2*>(q + at(v, 0)) = make_uint2(codes4(s[v][0], s[v][1], s[v][2], s[v][3], rs.inv),
+                                                                     codes4(s[v][4], s[v][5], s[v][6], s[v][7], rs.inv));
         } else {
 #pragma unroll
             for (int j = 0; j < 8; ++j)
-                if (at(v, j) < D) q[at(v, j)] = static_cast<int8_t>((j < 4 ? lo : hi) >> (8 * (j & 3)));
+                if (at(v, j) < left) q[at(v, j)] = static_cast<int8_t>(code_byte(s[v][j], rs.inv));
         }
     }
 }
