@@ -122,11 +122,11 @@ __global__ void __launch_bounds__(L ? 256 : 1024) rows_i8_kernel(const RowsI8 a)
     if (L && row - (threadIdx.x & 31) / (L ? L : 1) >= (size_t)a.M) return;
     const int D = row < (size_t)a.M ? a.D : 0;
     // This thread's first element, and the elements from there to the row's end: element j of vector v lies at(v, j)
-    // further on. Element by element a warp has 256 V neighbours, so that the distances are constants: what such a row
-    // costs is instructions.
+    // further on. Element by element a warp (or the part of it that has the row) has its neighbours, so that the
+    // distances are constants: what such a row costs is instructions.
     const int e0 = VEC ? 8 * t : L ? t : (t >> 5) * 256 * V + (t & 31);
     const int left = D - e0;
-    auto at = [&](int v, int j) { return VEC ? 8 * T * v + j : 256 * v + 32 * j; };
+    auto at = [&](int v, int j) { return VEC ? 8 * T * v + j : (L ? L : 32) * (8 * v + j); };
     const XT* __restrict__ x = static_cast<const XT*>(a.x) + row * a.ldx + e0;
     const DT* __restrict__ delta = static_cast<const DT*>(a.delta) + row * a.ldd + e0;
     const float* __restrict__ gp = NORM ? a.g + e0 : nullptr;

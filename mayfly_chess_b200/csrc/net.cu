@@ -1692,9 +1692,10 @@ static void launch_rows_i8_cfg(const RowsI8& a, int num_sms, cudaStream_t s)
 
 // Part of a warp up to 1,024 elements (2,048 for the 16-bit quantiser), then a block a row: as few threads as hold the
 // row with enough loads on their way. Measured (GB/s, 66,560 x 2,048 bf16 quantised: a warp of 8 vectors a thread 6,946,
-// a block of 2 5,843; 4,097 x 8,192 bf16 norm: blocks of 4 vectors 6,138, of 2 5,312, of 1 4,327). Rows that are read
-// element by element: 20,871 x 727 f16 quantised in a warp 2,829, in a block 1,978; 16,000 x 4,001 f16 norm in blocks of
-// 8 elements a thread 2,285, of 16 1,619, of 32 1,488, the quantiser there 1,822, 2,327 and 1,960.
+// a block of 2 5,843; 4,097 x 8,192 bf16 norm: blocks of 4 vectors 6,138, of 2 5,312, of 1 4,327). Element by
+// element: 20,871 x 727 f16 quantised in a warp 4,018, a block a row about half of that; 16,000 x 4,001 f16 norm in blocks
+// of 16 elements a thread 4,626, of 8 4,297, of 32 3,989, the quantiser there 4,407, 3,557 and 4,661, but 8,000 x 1,301
+// 3,141, 2,799 and 2,735; 45,120 x 70 bf16 norm in half a warp a row 2,202, in a warp 1,375.
 template <typename XT, typename DT, bool NORM>
 static void launch_rows_i8_t(const RowsI8& a, int num_sms, cudaStream_t s)
 {
@@ -1719,12 +1720,13 @@ static void launch_rows_i8_t(const RowsI8& a, int num_sms, cudaStream_t s)
         else if (D <= 16384) launch_rows_i8_cfg<XT, DT, NORM, true, 0, BV>(a, num_sms, s);
         else launch_rows_i8_cfg<XT, DT, NORM, true, 0, Q16 ? 8 : 4>(a, num_sms, s);
     } else {
-        constexpr int BV = NORM ? 1 : 2;
-        if (D <= 256) launch_rows_i8_cfg<XT, DT, NORM, false, 32, 1>(a, num_sms, s);
+        if (D <= 64) launch_rows_i8_cfg<XT, DT, NORM, false, 8, 1>(a, num_sms, s);
+        else if (D <= 128) launch_rows_i8_cfg<XT, DT, NORM, false, 16, 1>(a, num_sms, s);
+        else if (D <= 256) launch_rows_i8_cfg<XT, DT, NORM, false, 32, 1>(a, num_sms, s);
         else if (D <= 512) launch_rows_i8_cfg<XT, DT, NORM, false, 32, 2>(a, num_sms, s);
         else if (D <= 768) launch_rows_i8_cfg<XT, DT, NORM, false, 32, 3>(a, num_sms, s);
         else if (D <= 1024) launch_rows_i8_cfg<XT, DT, NORM, false, 32, 4>(a, num_sms, s);
-        else if (D <= 8192 * BV) launch_rows_i8_cfg<XT, DT, NORM, false, 0, BV>(a, num_sms, s);
+        else if (D <= (NORM ? 16384 : 2048)) launch_rows_i8_cfg<XT, DT, NORM, false, 0, 2>(a, num_sms, s);
         else launch_rows_i8_cfg<XT, DT, NORM, false, 0, 4>(a, num_sms, s);
     }
 }
