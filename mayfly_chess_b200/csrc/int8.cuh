@@ -300,6 +300,7 @@ struct I8Out {
     void* C;
     long long ldc;
     int M, N, K, n_tiles;
+    int direct;              // the pair kernel: C's rows are not whole 16-byte units, plain stores
 };
 
 // ------------------------------------------------------------------------------------------------ many rows
@@ -327,7 +328,7 @@ struct I8PairCfg {
 
 // A warp owns 32 rows of the tile and COLS neighbouring columns: it converts them from tensor memory into its own
 // staging chunk, and its lane 0 stores the chunk (for the residual: adds it at L2) by TMA, so that the warps of a group
-// meet once a tile and not at every chunk. The group's column scales and bias of a tile are read by its 128 threads a
+// meet once a tile and not at every chunk; where C does not suit TMA, the warp stores the chunk row by row. The group's column scales and bias of a tile are read by its 128 threads a
 // tile ahead and passed through shared memory: each is read once from L2, and an aligned float4 serves a warp.
 template <typename TO, int EPI, typename OriginFn, typename ReleaseFn>
 __device__ __forceinline__ void i8_pair_epilogue(const CUtensorMap* tmC, const I8Out& p, uint8_t* stages, float* vecs,
@@ -413,6 +414,33 @@ __device__ __forceinline__ void i8_pair_epilogue(const CUtensorMap* tmC, const I
             for (int j = 0; j < 4; ++j)
                 *reinterpret_cast<uint4*>(stage + swz<64>(lane, j)) =
                     make_uint4(q[4 * j], q[4 * j + 1], q[4 * j + 2], q[4 * j + 3]);
+            if (p.direct) {
+                // the warp's 32 x CHUNK values row by row, a row's columns by neighbouring lanes, eight stores' worth of a
+                // residual read at a time
+                __syncwarp();
+                constexpr int RPI = 32 / CHUNK;              // rows an instruction
+                const int cc = lane % CHUNK, n = col0 + c + cc, first = lane / CHUNK;
+                const int rows = n < p.N ? p.M - row0 : 0;
+                TO* cp = static_cast<TO*>(p.C) + (size_t)(row0 + first) * p.ldc + n;
+                const size_t step = RPI * (size_t)p.ldc;
+#pragma unroll 1
+                for (int i = 0; i < 32; i += 8 * RPI, cp += 8 * step) {
+                    TO v[8];
+#pragma unroll
+                    for (int u = 0; u < 8; ++u) {
+                        const int r = i + u * RPI + first;
+                        v[u] = *reinterpret_cast<const TO*>(stage + swz<64>(r, cc * (int)sizeof(TO) / 16) +
+                                                            cc * (int)sizeof(TO) % 16);
+                        if constexpr (EPI == kEpiResidual)
+                            if (r < rows) v[u] += cp[u * step];
+                    }
+#pragma unroll
+                    for (int u = 0; u < 8; ++u)
+                        if (i + u * RPI + first < rows) cp[u * step] = v[u];
+                }
+                __syncwarp();                                // read, before the next chunk overwrites it
+                continue;
+            }
             fence_proxy_async_smem();
             __syncwarp();
             if (lane == 0 && row0 < p.M) {
@@ -476,7 +504,7 @@ gemm_i8_pair_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_consta
         fence_barrier_init();
         tma_prefetch_desc(&tmA);
         tma_prefetch_desc(&tmW);
-        tma_prefetch_desc(&tmC);
+        if (!p.direct) tma_prefetch_desc(&tmC);
     }
     if (warp == 1) {
         tmem_alloc_pair(tmem_slot, 512);

@@ -1832,7 +1832,7 @@ static void launch_gemm_i8_split(const GemmI8& p, const CUtensorMap& mw, long lo
 // As many CTA pairs as can be resident at once, or as there are tiles.
 template <typename TO, int EPI>
 static void launch_gemm_i8_pair(const GemmI8& p, const CUtensorMap& ma, const CUtensorMap& mw, const CUtensorMap& mc,
-                                uint32_t* err, cudaStream_t s)
+                                bool direct, uint32_t* err, cudaStream_t s)
 {
     using C = I8PairCfg;
     static int max_pairs[64] = {};
@@ -1856,7 +1856,7 @@ static void launch_gemm_i8_pair(const GemmI8& p, const CUtensorMap& ma, const CU
     const long long tiles = (p.M + 255LL) / 256 * n_tiles;
     if (tiles > 0x7FFFFFFF) throw std::runtime_error("cudanet_k_gemm_i8: too many tiles");
     const int pairs = static_cast<int>(std::min<long long>(tiles, max_pairs[dev]));
-    const I8Out out{p.rowscale, p.colscale, p.bias, p.C, p.ldc, p.M, p.N, p.K, n_tiles};
+    const I8Out out{p.rowscale, p.colscale, p.bias, p.C, p.ldc, p.M, p.N, p.K, n_tiles, direct};
     launch_k(gemm_i8_pair_kernel<TO, EPI>, dim3(2 * pairs), dim3(C::THREADS), C::SMEM, s, ma, mw, mc, out, err);
 }
 
@@ -1867,13 +1867,12 @@ static void launch_gemm_i8_t(const GemmI8& p, int kernel, cudaStream_t s)
     RT(cudaGetDevice(&dev));
     RT(cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, dev));
     uint32_t* err = i8_error_word(dev);
-    // a TMA store writes whole 16-byte units, the last of a row past its end too: rows must be made of such units
+    // a TMA store writes whole 16-byte units, the last of a row past its end too: only for rows made of such units
     const bool units = reinterpret_cast<uintptr_t>(p.C) % 16 == 0 && p.N * sizeof(TO) % 16 == 0 &&
                        (p.M == 1 || p.ldc * sizeof(TO) % 16 == 0);
     I8SplitChoice choice{};
-    if (kernel != kI8Pair || !units) choice = pick_i8_split(p, sms);
+    if (kernel != kI8Pair) choice = pick_i8_split(p, sms);
     if (kernel < 0) kernel = choice.us <= i8_pair_us(p, sms) ? kI8Split : kI8Pair;
-    if (!units && kernel == kI8Pair) kernel = kI8Split;
     const auto pitch = [](long long ld, int width, int rows) { return rows > 1 ? ld : (width + 15LL) / 16 * 16; };
     const long long pa = pitch(p.lda, p.K, p.M);
     const CUtensorMap mw = make_map(p.W, MapType::U8, p.K, p.N, pitch(p.ldw, p.K, p.N), 128, 128);
@@ -1891,8 +1890,9 @@ static void launch_gemm_i8_t(const GemmI8& p, int kernel, cudaStream_t s)
     constexpr MapType t = std::is_same<TO, float>::value    ? MapType::F32
                           : std::is_same<TO, __half>::value ? MapType::F16
                                                             : MapType::BF16;
-    const CUtensorMap mc = make_map(p.C, t, p.N, p.M, pitch(p.ldc, p.N, p.M), 64 / sizeof(TO), 32, true);
-    launch_gemm_i8_pair<TO, EPI>(p, ma, mw, mc, err, s);
+    // with plain stores the kernel does not use the output's map: any valid one
+    const CUtensorMap mc = units ? make_map(p.C, t, p.N, p.M, pitch(p.ldc, p.N, p.M), 64 / sizeof(TO), 32, true) : ma;
+    launch_gemm_i8_pair<TO, EPI>(p, ma, mw, mc, !units, err, s);
 }
 
 // A null pointer, or one whose address is no multiple of `align`, named in the reason.
