@@ -1793,6 +1793,17 @@ static double i8_pair_us(const GemmI8& p, int num_sms)
     return 4.5 + rounds * (1.8 + 0.28 * ((p.K + 127) / 128));
 }
 
+// Outputs whose rows are not whole 16-byte units: the least time (us) that their stores take, whatever K is. Millions of
+// elements a millisecond, from 66,560 x 2,047 x 128 (pairs 152 us in bf16, 313 in f32; split 160 and 151) and, added to
+// f32, 15,232 x 2,937 x 1,861 (131 and 172; 27,690 x 2,993 x 848: 212 and 177): a pair's warp writes 64 bytes of a row at
+// once, a split tile's 128 of f32.
+static double i8_plain_store_us(const GemmI8& p, int epi, bool pair)
+{
+    const double rate = epi == kEpiResidual ? (pair ? 400. : 260.) : epi == kEpiF32 ? (pair ? 435. : 900.)
+                                                                                     : (pair ? 900. : 850.);
+    return double(p.M) * p.N / (rate * 1e3);
+}
+
 template <typename TO, int EPI, int TN>
 static void launch_gemm_i8_split(const GemmI8& p, const CUtensorMap& mw, long long pitch_a, int split, uint32_t* err,
                                  cudaStream_t s)
@@ -1872,7 +1883,14 @@ static void launch_gemm_i8_t(const GemmI8& p, int kernel, cudaStream_t s)
                        (p.M == 1 || p.ldc * sizeof(TO) % 16 == 0);
     I8SplitChoice choice{};
     if (kernel != kI8Pair) choice = pick_i8_split(p, sms);
-    if (kernel < 0) kernel = choice.us <= i8_pair_us(p, sms) ? kI8Split : kI8Pair;
+    if (kernel < 0) {
+        double split_us = choice.us, pair_us = i8_pair_us(p, sms);
+        if (!units) {
+            split_us = std::max(split_us, i8_plain_store_us(p, EPI, false));
+            pair_us = std::max(pair_us, i8_plain_store_us(p, EPI, true));
+        }
+        kernel = split_us <= pair_us ? kI8Split : kI8Pair;
+    }
     const auto pitch = [](long long ld, int width, int rows) { return rows > 1 ? ld : (width + 15LL) / 16 * 16; };
     const long long pa = pitch(p.lda, p.K, p.M);
     const CUtensorMap mw = make_map(p.W, MapType::U8, p.K, p.N, pitch(p.ldw, p.K, p.N), 128, 128);
