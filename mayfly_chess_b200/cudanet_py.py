@@ -668,15 +668,17 @@ def k_rmsnorm_i8(x, delta, g, out, q, scale, eps=1e-6, dll=None):
     scale)."""
     once = _i8_once or _i8_setup()
     f32, shape, dev, xt = once.f32, x.shape, x.get_device(), _i8_type(once, x, "x")
-    xs, qs = x.stride(), q.stride()
-    if (len(shape) != 2 or dev < 0 or xs[1] != 1 or q.dtype is not once.int8 or q.shape != shape or qs[1] != 1
-            or q.get_device() != dev or g.dtype is not f32 or g.shape != shape[1:] or g.get_device() != dev
-            or not g.is_contiguous() or scale.dtype is not f32 or scale.shape != shape[:1]
-            or scale.get_device() != dev or not scale.is_contiguous()):
+    if len(shape) != 2:
+        _i8_matrix(x, "x", shape, dev)
+    (M, D), xs, qs = shape, x.stride(), q.stride()
+    if (dev < 0 or xs[1] != 1 or q.dtype is not once.int8 or q.shape != shape or qs[1] != 1 or q.get_device() != dev
+            or g.dtype is not f32 or g.shape != (D,) or g.get_device() != dev or not g.is_contiguous()
+            or scale.dtype is not f32 or scale.shape != (M,) or scale.get_device() != dev
+            or not scale.is_contiguous()):
         _i8_matrix(x, "x", shape, dev)
         _i8_matrix(q, "q", shape, dev, once.int8)
-        _i8_vector(once, g, "g", shape[1], dev)
-        _i8_vector(once, scale, "scale", shape[0], dev)
+        _i8_vector(once, g, "g", D, dev)
+        _i8_vector(once, scale, "scale", M, dev)
     if delta is None:
         if out is not None:
             raise ValueError("out without delta: there is no sum to store")
@@ -696,8 +698,8 @@ def k_rmsnorm_i8(x, delta, g, out, q, scale, eps=1e-6, dll=None):
             return k_rmsnorm_i8(x, delta, g, out, q, scale, eps, dll)
     reason = _i8_reason.buffer
     if (once.lib if dll is None and once.lib else once.load(dll)).cudanet_k_rmsnorm_i8(
-            xt, dt, x.data_ptr(), dp, g.data_ptr(), op, q.data_ptr(), scale.data_ptr(), shape[0], shape[1], xs[0], ldd,
-            ldo, qs[0], eps, once.stream(dev), reason, ERR_LEN) != 0:
+            xt, dt, x.data_ptr(), dp, g.data_ptr(), op, q.data_ptr(), scale.data_ptr(), M, D, xs[0], ldd, ldo,
+            qs[0], eps, once.stream(dev), reason, ERR_LEN) != 0:
         raise RuntimeError(f"cudanet_k_rmsnorm_i8: {_msg(reason)}")
     return q, scale
 
@@ -708,19 +710,21 @@ def k_quant_i8(x, q, scale, dll=None):
     the device's current stream. Returns (q, scale)."""
     once = _i8_once or _i8_setup()
     shape, dev, xt = x.shape, x.get_device(), _i8_type(once, x, "x")
-    xs, qs = x.stride(), q.stride()
-    if (len(shape) != 2 or dev < 0 or xs[1] != 1 or q.dtype is not once.int8 or q.shape != shape or qs[1] != 1
-            or q.get_device() != dev or scale.dtype is not once.f32 or scale.shape != shape[:1]
-            or scale.get_device() != dev or not scale.is_contiguous()):
+    if len(shape) != 2:
+        _i8_matrix(x, "x", shape, dev)
+    (M, D), xs, qs = shape, x.stride(), q.stride()
+    if (dev < 0 or xs[1] != 1 or q.dtype is not once.int8 or q.shape != shape or qs[1] != 1 or q.get_device() != dev
+            or scale.dtype is not once.f32 or scale.shape != (M,) or scale.get_device() != dev
+            or not scale.is_contiguous()):
         _i8_matrix(x, "x", shape, dev)
         _i8_matrix(q, "q", shape, dev, once.int8)
-        _i8_vector(once, scale, "scale", shape[0], dev)
+        _i8_vector(once, scale, "scale", M, dev)
     if once.device() != dev:
         with once.on_device(dev):
             return k_quant_i8(x, q, scale, dll)
     reason = _i8_reason.buffer
     if (once.lib if dll is None and once.lib else once.load(dll)).cudanet_k_quant_i8(
-            xt, x.data_ptr(), q.data_ptr(), scale.data_ptr(), shape[0], shape[1], xs[0], qs[0], once.stream(dev),
+            xt, x.data_ptr(), q.data_ptr(), scale.data_ptr(), M, D, xs[0], qs[0], once.stream(dev),
             reason, ERR_LEN) != 0:
         raise RuntimeError(f"cudanet_k_quant_i8: {_msg(reason)}")
     return q, scale
@@ -741,8 +745,8 @@ def k_gemm_i8(A, W, rowscale, colscale, bias, C, epi, kernel=-1, dll=None):
     ta, tw, tc = A.stride(), W.stride(), C.stride()
     if (dev < 0 or A.dtype is not i8 or ta[1] != 1 or W.dtype is not i8 or tw[1] != 1 or W.get_device() != dev
             or C.shape != (M, N) or tc[1] != 1 or C.get_device() != dev or rowscale.dtype is not f32
-            or rowscale.shape != sa[:1] or rowscale.get_device() != dev or not rowscale.is_contiguous()
-            or colscale.dtype is not f32 or colscale.shape != sw[:1] or colscale.get_device() != dev
+            or rowscale.shape != (M,) or rowscale.get_device() != dev or not rowscale.is_contiguous()
+            or colscale.dtype is not f32 or colscale.shape != (N,) or colscale.get_device() != dev
             or not colscale.is_contiguous()):
         _i8_matrix(A, "A", sa, dev, i8)
         _i8_matrix(W, "W", sw, dev, i8)
@@ -751,7 +755,7 @@ def k_gemm_i8(A, W, rowscale, colscale, bias, C, epi, kernel=-1, dll=None):
         _i8_vector(once, colscale, "colscale", N, dev)
     bp = None
     if bias is not None:
-        if (bias.dtype is not f32 or bias.shape != sw[:1] or bias.get_device() != dev or not bias.is_contiguous()):
+        if (bias.dtype is not f32 or bias.shape != (N,) or bias.get_device() != dev or not bias.is_contiguous()):
             _i8_vector(once, bias, "bias", N, dev)
         bp = bias.data_ptr()
     if once.device() != dev:
