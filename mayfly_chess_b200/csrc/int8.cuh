@@ -312,7 +312,7 @@ struct I8Out {
 // What paced the products before was their issue: by one lane of a diverged warp, with two commits a stage, 187 cycles an
 // instruction; from a converged warp with one commit to both CTAs 128 to 140 (66,560 x 2,048 x 1,024: 131 -> 113 us).
 // What bounds it now: 8,192^3 keeps the tensor cores busy 92% of their cycles (2,630 TOP/s); the 1,000 W cap, which takes
-// the clock from 1.97 to about 1.4 GHz in a long run (66,560 x 2,048 x 1,024 there 134 us, with GELU 147); and with GELU
+// the clock from 1.97 to about 1.4 GHz in a long run (66,560 x 2,048 x 1,024 there 134 us, with GELU 147 to 150; cool 109 and 122); and with GELU
 // the epilogue's instructions (7,100 cycles a tile against 6,100 without it and 4,096 of products). Roles: warp 0 TMA
 // loads, warp 1 tensor memory and the products (leader CTA), warps 2..17 the epilogue.
 struct I8PairCfg {
@@ -376,7 +376,7 @@ __device__ __forceinline__ void i8_pair_epilogue(const CUtensorMap* tmC, const I
             uint32_t a[LD], q[16];
             if constexpr (LD == 32) tmem_ld_32x32b_x32(t_acc + static_cast<uint32_t>(c), a);
             else tmem_ld_32x32b_x16(t_acc + static_cast<uint32_t>(c), a);
-            tmem_ld_wait();
+            tmem_ld_wait(a);
             if (c == COLS - CHUNK) {
                 tc_fence_before();
                 __syncwarp();
@@ -763,7 +763,7 @@ gemm_i8_split_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_const
             if constexpr (LD == 4) tmem_ld_32x32b_x4(t_lane + static_cast<uint32_t>(t0), a);
             else if constexpr (LD == 8) tmem_ld_32x32b_x8(t_lane + static_cast<uint32_t>(t0), a);
             else tmem_ld_32x32b_x16(t_lane + static_cast<uint32_t>(t0), a);
-            tmem_ld_wait();
+            tmem_ld_wait(a);
             if (S > 1) {
 #pragma unroll
                 for (int i = 0; i < LD; ++i) part[(t0 + i) * 128 + n_in] = static_cast<int>(a[i]);

@@ -432,6 +432,14 @@ __device__ __forceinline__ void tmem_ld_32x32b_x32(uint32_t taddr, uint32_t (&r)
 
 __device__ __forceinline__ void tmem_ld_wait() { asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory"); }
 
+// The same, with the registers that the loads fill: their uses stay behind the wait.
+template <int N> __device__ __forceinline__ void tmem_ld_wait(uint32_t (&r)[N])
+{
+    tmem_ld_wait();
+#pragma unroll
+    for (int i = 0; i < N; ++i) asm volatile("" : "+r"(r[i]));
+}
+
 // the reverse: thread t of the warp writes lane (base lane + t), columns col..col+31
 __device__ __forceinline__ void tmem_st_32x32b_x32(uint32_t taddr, const uint32_t (&r)[32])
 {
