@@ -312,9 +312,9 @@ struct I8Out {
 // What paced the products before was their issue: by one lane of a diverged warp, with two commits a stage, 187 cycles an
 // instruction; from a converged warp with one commit to both CTAs 128 to 140 (66,560 x 2,048 x 1,024: 131 -> 113 us).
 // What bounds it now: 8,192^3 keeps the tensor cores busy 92% of their cycles (2,630 TOP/s); the 1,000 W cap, which takes
-// the clock from 1.97 to about 1.4 GHz in a long run (66,560 x 2,048 x 1,024 there 134 us, with GELU 147 to 150; cool 109 and 122); and with GELU
-// the epilogue's instructions (7,100 cycles a tile against 6,100 without it and 4,096 of products). Roles: warp 0 TMA
-// loads, warp 1 tensor memory and the products (leader CTA), warps 2..17 the epilogue.
+// the clock from 1.97 to about 1.4 GHz in a long run (66,560 x 2,048 x 1,024 there 134 us, with GELU 147 to 150; cool 109
+// and 122); and with GELU the epilogue's instructions (7,100 cycles a tile against 6,100 without it and 4,096 of
+// products). Roles: warp 0 TMA loads, warp 1 tensor memory and the products (leader CTA), warps 2..17 the epilogue.
 struct I8PairCfg {
     static constexpr int SLOTS = 11;                     // of 128 rows x 128 bytes
     static constexpr uint32_t SLOT = 128 * 128;
