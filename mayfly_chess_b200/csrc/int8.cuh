@@ -111,7 +111,7 @@ __device__ __forceinline__ uint32_t codes4(float a, float b, float c, float d, f
 // 110 us, 6.8 TB/s; quantiser 66,560 x 2,048 bf16: 59 us, 6.9 TB/s). VEC: neighbouring elements 8 at a
 // time (D a multiple of 8, every row of every operand begins on 16 bytes, q's on 8); else element by element.
 template <typename XT, typename DT, bool NORM, bool VEC, int L, int V>
-__global__ void __launch_bounds__(L ? 256 : 1024) rows_i8_kernel(const RowsI8 a)
+__global__ void __launch_bounds__(L ? 128 : 1024) rows_i8_kernel(const RowsI8 a)
 {
     griddep_wait();
     griddep_launch();
