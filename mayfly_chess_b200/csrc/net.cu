@@ -1770,16 +1770,22 @@ struct I8SplitChoice {
     int tokens, split;
     double us;
 };
+// Rows of operands that do not begin on 128 bytes: a block of K then takes two lines of L2 a row, and the models below
+// count its loads 1.9 and 1.2 times (3,000 x 1,000 x 1,000: 9.2 us in pairs, 11.1 split; 1,017 x 1,272 x 3,975 17.3 and
+// 20.0; 300 x 1,000 x 3,000: 7.3 us in tiles of 64 tokens with K split in 4, 9.2 in tiles of 16 unsplit).
+static bool i8_uneven(const GemmI8& p) { return (p.M > 1 && p.lda % 128) || (p.N > 1 && p.ldw % 128); }
+
 static I8SplitChoice pick_i8_split(const GemmI8& p, int num_sms)
 {
     const int blocks = (p.K + 127) / 128;
+    const double load = i8_uneven(p) ? 1.9 : 1.;
     I8SplitChoice best{128, 1, 1e30};
     for (int TN : {16, 32, 64, 128}) {
         const double tiles = std::ceil(p.N / 128.) * std::ceil(p.M / double(TN)), share = std::min(p.M, TN);
         for (int S = 1; S <= 8 && S <= blocks; S *= 2) {
             const double ctas = tiles * S, of_k = (blocks + S - 1) / S, rounds = std::ceil(ctas / (2. * num_sms));
-            const double us = 1.73 + rounds * (0.267 * of_k + 0.0216 * share + (S > 1 ? 0.67 : 0.)) +
-                              0.0141e-6 * 128. * of_k * (128. + share) * ctas + (S > 1 ? 1.53 * ctas / num_sms : 0.);
+            const double us = 1.73 + rounds * (0.267 * load * of_k + 0.0216 * share + (S > 1 ? 0.67 : 0.)) +
+                              0.0141e-6 * 128. * load * of_k * (128. + share) * ctas + (S > 1 ? 1.53 * ctas / num_sms : 0.);
             if (us < best.us) best = {TN, S, us};
         }
     }
@@ -1791,7 +1797,7 @@ static I8SplitChoice pick_i8_split(const GemmI8& p, int num_sms)
 static double i8_pair_us(const GemmI8& p, int num_sms)
 {
     const double rounds = std::ceil(std::ceil(p.M / 256.) * std::ceil(p.N / 256.) / (num_sms / 2));
-    return 4.5 + rounds * (1.8 + 0.28 * ((p.K + 127) / 128));
+    return 4.5 + rounds * (1.8 + 0.28 * (i8_uneven(p) ? 1.2 : 1.) * ((p.K + 127) / 128));
 }
 
 // Outputs whose rows are not whole 16-byte units: the least time (us) that their stores take, whatever K is. Millions of
