@@ -208,9 +208,9 @@ CUDANET_API int cudanet_k_layernorm_f8(int x_dtype, const void* x, const float* 
  * a result nor written. M = 0 does nothing; M <= 2^30. Outputs overlap no other argument, save where it is said. A
  * process' first call of each kind loads its kernel. Return 0, or -1 with the reason in err.
  *
- * A row's codes are q[i] = rint(t[i] * (127 / a)) (ties to even), a = max |t[i]|, so that -127 <= q <= 127. A row
- * with a < 2^-120 has scale 0 and codes 0. A row that holds a NaN or an infinity (for the norm: or whose sum of
- * squares leaves f32) has scale NaN and codes 0, so every product of it is NaN. */
+ * A row's codes are q[i] = rint(127 t[i] / a), the quotient in f32, ties to even, a = max |t[i]|, so that
+ * -127 <= q <= 127. A row with a < 2^-120 has scale 0 and codes 0. A row that holds a NaN or an infinity (for the
+ * norm: or whose sum of squares leaves f32) has scale NaN and codes 0, so every product of it is NaN. */
 
 /* out = x + delta rounded to x's type (delta of x's type, or of any type where x is f32; out may be x or, of the same
  * type, delta); then the codes of t = out * g and scale = a / sqrt(mean(out^2) + eps) / 127: q * scale stands for

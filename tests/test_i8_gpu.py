@@ -187,6 +187,38 @@ def test_codes_at_the_ties(k):
     assert scale[0] == 1 and torch.equal(q.float(), torch.round(X))
 
 
+@pytest.mark.parametrize("x", ["f32", "bf16", "f16"])
+@pytest.mark.parametrize("D,off", [(8, 0), (8, 1), (727, 1), (1024, 0), (2048, 0), (2048, 1), (4104, 0)])
+def test_codes_of_half_the_largest(k, x, D, off):
+    """Half of a row's largest is 63.5 steps, a tie, whatever the largest is: code 64, the even one. Here the largest
+    takes every bf16 mantissa."""
+    a = ((1 + torch.arange(128, device="cuda") / 128) * 2.0 ** (torch.arange(128, device="cuda") % 9 - 4))[:, None]
+    sign = torch.where(torch.arange(D, device="cuda") % 3 == 0, -1.0, 1.0)
+    X, _ = matrix(128, D, DT[x], D, 0, off)
+    X.copy_(sign * a / 2)
+    X[:, D // 2] = a[:, 0].to(DT[x])
+    want = 64 * sign.expand(128, D).clone()
+    want[:, D // 2] = 127
+    q, scale = torch.empty(128, D, dtype=torch.int8, device="cuda"), torch.empty(128, device="cuda")
+    k.k_quant_i8(X, q, scale)
+    assert torch.equal(q.float(), want)
+    k.k_rmsnorm_i8(X, None, torch.ones(D, device="cuda"), None, q, scale)
+    assert torch.equal(q.float(), want)
+
+
+@pytest.mark.parametrize("x", ["f32", "bf16", "f16"])
+@pytest.mark.parametrize("M,D,off", [(2000, 2048, 0), (1000, 1001, 0), (300, 8192, 0), (5000, 130, 1)])
+def test_codes_are_the_rounded_quotient(k, x, M, D, off):
+    """A code is 127 t / max |t| in f32, rounded to a whole number, ties to even. In 64 bits the quotient has 29 bits
+    more than it is then rounded to."""
+    X, _ = matrix(M, D, DT[x], D, 0, off)
+    X.copy_(torch.randn(M, D, device="cuda", generator=gen(D)))
+    q, scale = torch.empty(M, D, dtype=torch.int8, device="cuda"), torch.empty(M, device="cuda")
+    k.k_quant_i8(X, q, scale)
+    t = X.double()
+    assert torch.equal(q.float(), torch.round((127 * t / t.abs().amax(1, keepdim=True)).float()))
+
+
 # ------------------------------------------------------------------------------------------------ product
 def operands(M, N, K, seed, full=False):
     """Codes whose rows begin on 16 bytes, what lies behind them filled with codes that must not count."""
