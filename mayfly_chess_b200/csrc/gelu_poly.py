@@ -22,19 +22,19 @@ NODES = 4000
 A_MAX = 10.0
 
 
-def coefficients(degree=DEGREE, nodes=NODES, a_max=A_MAX):
-    """Monomial coefficients c[0..degree] of P(u) ~ log2 Phi(-(a_max / 2) (u + 1)), lowest power first."""
+def coefficients(degree=DEGREE, nodes=NODES):
+    """Monomial coefficients c[0..degree] of P(u) ~ log2 Phi(-5 (u + 1)), lowest power first."""
     k = np.arange(nodes)
     u = np.cos(np.pi * (k + 0.5) / nodes)
-    a = (a_max / 2) * (u + 1)
+    a = (A_MAX / 2) * (u + 1)
     cheb = np.polynomial.chebyshev.chebfit(u, log_ndtr(-a) / np.log(2), degree)
     return np.polynomial.chebyshev.cheb2poly(cheb)
 
 
-def float32_error(c, samples=400001, a_max=A_MAX):
-    """max relative error of 2^P(u) against q(a) over a in [0, a_max], P evaluated in float32."""
-    a = np.linspace(0, a_max, samples).astype(np.float32)
-    u = (a * np.float32(2 / a_max) + np.float32(-1)).astype(np.float32)
+def float32_error(c, samples=400001):
+    """max relative error of 2^P(u) against q(a) over a in [0, A_MAX], P evaluated in float32."""
+    a = np.linspace(0, A_MAX, samples).astype(np.float32)
+    u = (a * np.float32(2 / A_MAX) + np.float32(-1)).astype(np.float32)
     c32 = c.astype(np.float32)
     p = np.full_like(u, c32[-1])
     for ci in c32[-2::-1]:
@@ -44,9 +44,7 @@ def float32_error(c, samples=400001, a_max=A_MAX):
 
 
 if __name__ == "__main__":
-    # gemm.cuh's, and the int8 products' for bf16 outputs (int8.cuh)
-    for degree, a_max in ((DEGREE, A_MAX), (6, 8.0)):
-        c = coefficients(degree, a_max=a_max)
-        for i, v in enumerate(c):
-            print(f"c{i} = {np.float32(v)!r:>16}  ({v:.12e})")
-        print(f"max relative error of q in float32 over [0, {a_max:g}]: {float32_error(c, a_max=a_max):.3e}")
+    c = coefficients()
+    for i, v in enumerate(c):
+        print(f"c{i} = {np.float32(v)!r:>16}  ({v:.12e})")
+    print(f"max relative error of q in float32 over [0, {A_MAX:g}]: {float32_error(c):.3e}")

@@ -298,29 +298,6 @@ __device__ __forceinline__ float i8_value(int acc, float rowscale, float colscal
     return fmaf(__fmul_rn(__int2float_rn(acc), rowscale), colscale, bias);
 }
 
-// GELU of two values for an output of type TO, NaN for a NaN. bf16: gelu_pair's form with a polynomial of degree 6 in
-// u = a / 4 - 1, a = min(|x|, 8) (gelu_poly.py), whose relative error of q, 2.6e-4, is a fifteenth of the half step
-// that the output is rounded by (2^-8) and which saves two of eleven fused steps; f16, with a half step of 2^-11: gelu_pair.
-template <typename TO> __device__ __forceinline__ float2 gelu_i8(uint64_t x2)
-{
-    if constexpr (std::is_same<TO, __nv_bfloat16>::value) {
-        const auto both = [](float v) { return pk2(v, v); };
-        const float2 x = upk2(x2);
-        const uint64_t na = pk2(fmaxf(-fabsf(x.x), -8.0f), fmaxf(-fabsf(x.y), -8.0f));
-        const uint64_t u = fma2(na, both(-0.25f), both(-1.0f));
-        uint64_t p = fma2(u, both(5.278726295e-02f), both(-1.125788987e-01f));
-        p = fma2(u, p, both(1.381741464e-01f));
-        p = fma2(u, p, both(-2.566262186e-01f));
-        p = fma2(u, p, both(-1.100134087e+01f));
-        p = fma2(u, p, both(-2.438733101e+01f));
-        p = fma2(u, p, both(-1.494651318e+01f));
-        const float2 l = upk2(p);
-        return upk2(fma2(na, pk2(ex2_approx_f(l.x), ex2_approx_f(l.y)), pk2(relu_nan(x.x), relu_nan(x.y))));
-    } else {
-        return gelu_pair<false, true>(x2, GeluK(1.0f));
-    }
-}
-
 // The outputs and vectors of a product.
 struct I8Out {
     const float *rowscale, *colscale, *bias;
@@ -419,8 +396,8 @@ __device__ __forceinline__ void i8_pair_epilogue(const CUtensorMap* tmC, const I
                                          pk2(sc.z, sc.w), pk2(b.z, b.w));
                 float2 x, y;
                 if constexpr (EPI == kEpiBiasGelu) {
-                    x = gelu_i8<TO>(lo);
-                    y = gelu_i8<TO>(hi);
+                    x = gelu_pair<false, true>(lo, GeluK(1.0f));
+                    y = gelu_pair<false, true>(hi, GeluK(1.0f));
                 } else {
                     x = upk2(lo);
                     y = upk2(hi);
@@ -716,7 +693,7 @@ gemm_i8_split_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_const
     // the outputs of tokens t and u from their accumulators; a token outside [0, end) is computed and not stored
     const auto put2 = [&](int acc_t, int t, int acc_u, int u, int end) {
         float2 v = make_float2(i8_value(acc_t, s_rowscale[t], cs, bias), i8_value(acc_u, s_rowscale[u], cs, bias));
-        if constexpr (EPI == kEpiBiasGelu) v = gelu_i8<TO>(pk2(v.x, v.y));
+        if constexpr (EPI == kEpiBiasGelu) v = gelu_pair<false, true>(pk2(v.x, v.y), GeluK(1.0f));
         TO *ct = c + (size_t)t * p.ldc, *cu = c + (size_t)u * p.ldc;
         if constexpr (EPI == kEpiResidual) {   // added at L2, once an element: nothing waits for the old value
             if (t < end) atomicAdd(ct, v.x);

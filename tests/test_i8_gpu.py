@@ -310,6 +310,23 @@ def test_gemm_nan_scale_marks_its_row(k):
             assert bad[3].all() and not bad[[i for i in range(70) if i != 3]].any()
 
 
+@pytest.mark.parametrize("out", ["bf16", "f16"])
+def test_gelu_of_every_size(k, out):
+    """The products are zero here, so an output is gelu(bias). It lies between the roundings of the exact value less and
+    plus what the GELU before it may be off by: 2.5e-5 of |x| Phi(-|x|) (the polynomial), four roundings of f32, and
+    1e-22 below x = -10, where Phi is held."""
+    N = 1 << 18
+    x = torch.linspace(-12, 12, N, device="cuda")
+    A, W = torch.zeros(2, 16, dtype=torch.int8, device="cuda"), torch.zeros(N, 16, dtype=torch.int8, device="cuda")
+    d = x.double()
+    v = d * torch.special.erfc(-d / math.sqrt(2)) / 2              # erfc keeps the far negative side, ndtr gives 0 there
+    e = 2.5e-5 * d.abs() * torch.special.erfc(d.abs() / math.sqrt(2)) / 2 + 4 * U * v.abs() + 1e-22
+    C = torch.empty(2, N, dtype=DT[out], device="cuda")
+    for kernel in (1, 2):
+        k.k_gemm_i8(A, W, torch.ones(2, device="cuda"), torch.ones(N, device="cuda"), x, C, 1, kernel)
+        assert (C >= (v - e).to(C.dtype)).all() and (C <= (v + e).to(C.dtype)).all(), kernel
+
+
 def test_gemm_offset_vectors(k):
     """Scales and bias that begin on 4 bytes, and operands that are rows of larger matrices."""
     A, W, rs, cs, bias = operands(400, 520, 256, 9)
