@@ -232,7 +232,9 @@ CUDANET_API int cudanet_k_quant_i8(int x_type, const void* x, void* q, float* sc
  * CTA pairs, 2 for the kernel with weights on the tensor cores' lanes and K split as it chooses, 3, 4, 6 and 10 for that
  * with K split over 1, 2, 4 and 8 CTAs (fewer where K has fewer blocks of 128). Every kernel gives the same bits (epi 2
  * adds once an element in L2, which may take a sum below the smallest normal f32 for 0). A wait inside the kernel that runs
- * out (a failure of the device) ends it with C partly unwritten and is reported by cudanet_k_i8_check. */
+ * out (a failure of the device) ends it with C partly unwritten, never with a sum that lacks a part, and is reported by
+ * cudanet_k_i8_check. For tests, 67, 68, 70 and 74 are 3, 4, 6 and 10 with no operands for each cluster's last CTA, whose
+ * waits run out after 2 s: nothing is stored. */
 CUDANET_API int cudanet_k_gemm_i8(int dtype, int epi, int kernel, const void* A, const void* W, const float* rowscale,
                                   const float* colscale, const float* bias, void* C, int M, int N, int K, int64_t lda,
                                   int64_t ldw, int64_t ldc, void* stream, char* err, int err_len);

@@ -1757,7 +1757,7 @@ struct GemmI8 {
 };
 
 // The kernels of an int8 product: the choice of `kernel` -1, else what the caller asks for.
-enum I8Kernel : int { kI8Pair = 1, kI8Split = 2 };   // kI8Split + S: the split over S CTAs
+enum I8Kernel : int { kI8Pair = 1, kI8Split = 2, kI8Stall = 64 };   // kI8Split + S: the split over S CTAs
 
 // The split kernel's tokens a tile and CTAs a tile, and its time by the model that chooses them (us): a start, then for
 // each round of CTAs (two an SM at once) a CTA's 128-byte blocks of K, its tokens' epilogue and the exchange of a split,
@@ -1812,8 +1812,8 @@ static double i8_plain_store_us(const GemmI8& p, int epi, bool pair)
 }
 
 template <typename TO, int EPI, int TN>
-static void launch_gemm_i8_split(const GemmI8& p, const CUtensorMap& mw, long long pitch_a, int split, uint32_t* err,
-                                 cudaStream_t s)
+static void launch_gemm_i8_split(const GemmI8& p, const CUtensorMap& mw, long long pitch_a, int split, bool stall,
+                                 uint32_t* err, cudaStream_t s)
 {
     using C = I8SplitCfg<TN>;
     static bool attr[64] = {};
@@ -1843,7 +1843,7 @@ static void launch_gemm_i8_split(const GemmI8& p, const CUtensorMap& mw, long lo
     la[1].val.clusterDim.y = la[1].val.clusterDim.z = 1;
     cfg.attrs = la;
     cfg.numAttrs = 2;
-    const I8Out out{p.rowscale, p.colscale, p.bias, p.C, p.ldc, p.M, p.N, p.K, n_tiles};
+    const I8Out out{p.rowscale, p.colscale, p.bias, p.C, p.ldc, p.M, p.N, p.K, n_tiles, 0, stall};
     RT(cudaLaunchKernelEx(&cfg, gemm_i8_split_kernel<TO, EPI, TN>, ma, mw, out, err));
 }
 
@@ -1874,7 +1874,7 @@ static void launch_gemm_i8_pair(const GemmI8& p, const CUtensorMap& ma, const CU
     const long long tiles = (p.M + 255LL) / 256 * n_tiles;
     if (tiles > 0x7FFFFFFF) throw std::runtime_error("cudanet_k_gemm_i8: too many tiles");
     const int pairs = static_cast<int>(std::min<long long>(tiles, max_pairs[dev]));
-    const I8Out out{p.rowscale, p.colscale, p.bias, p.C, p.ldc, p.M, p.N, p.K, n_tiles, direct};
+    const I8Out out{p.rowscale, p.colscale, p.bias, p.C, p.ldc, p.M, p.N, p.K, n_tiles, direct, 0};
     launch_k(gemm_i8_pair_kernel<TO, EPI>, dim3(2 * pairs), dim3(C::THREADS), C::SMEM, s, ma, mw, mc, out, err);
 }
 
@@ -1885,6 +1885,8 @@ static void launch_gemm_i8_t(const GemmI8& p, int kernel, cudaStream_t s)
     RT(cudaGetDevice(&dev));
     RT(cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, dev));
     uint32_t* err = i8_error_word(dev);
+    const bool stall = kernel >= kI8Stall;
+    if (stall) kernel -= kI8Stall;
     // a TMA store writes whole 16-byte units, the last of a row past its end too: only for rows made of such units
     const bool units = reinterpret_cast<uintptr_t>(p.C) % 16 == 0 && p.N * sizeof(TO) % 16 == 0 &&
                        (p.M == 1 || p.ldc * sizeof(TO) % 16 == 0);
@@ -1904,10 +1906,10 @@ static void launch_gemm_i8_t(const GemmI8& p, int kernel, cudaStream_t s)
     if (kernel >= kI8Split) {
         const int split = kernel > kI8Split ? kernel - kI8Split : choice.split;
         switch (choice.tokens) {
-            case 16: launch_gemm_i8_split<TO, EPI, 16>(p, mw, pa, split, err, s); break;
-            case 32: launch_gemm_i8_split<TO, EPI, 32>(p, mw, pa, split, err, s); break;
-            case 64: launch_gemm_i8_split<TO, EPI, 64>(p, mw, pa, split, err, s); break;
-            default: launch_gemm_i8_split<TO, EPI, 128>(p, mw, pa, split, err, s);
+            case 16: launch_gemm_i8_split<TO, EPI, 16>(p, mw, pa, split, stall, err, s); break;
+            case 32: launch_gemm_i8_split<TO, EPI, 32>(p, mw, pa, split, stall, err, s); break;
+            case 64: launch_gemm_i8_split<TO, EPI, 64>(p, mw, pa, split, stall, err, s); break;
+            default: launch_gemm_i8_split<TO, EPI, 128>(p, mw, pa, split, stall, err, s);
         }
         return;
     }
@@ -2505,7 +2507,8 @@ CUDANET_API int cudanet_k_gemm_i8(int dtype, int epi, int kernel, const void* A,
         const char* who = "cudanet_k_gemm_i8";
         if (dtype != 0 && dtype != 1) throw std::runtime_error(std::string(who) + ": dtype must be 0 (f16) or 1 (bf16)");
         if (epi < 0 || epi > 3) throw std::runtime_error(std::string(who) + ": epi must be 0..3");
-        if (kernel != -1 && kernel != 1 && kernel != 2 && kernel != 3 && kernel != 4 && kernel != 6 && kernel != 10)
+        const int of = kernel >= mf::kI8Stall + 3 ? kernel - mf::kI8Stall : kernel;
+        if (of != -1 && of != 1 && of != 2 && of != 3 && of != 4 && of != 6 && of != 10)
             throw std::runtime_error(std::string(who) + ": kernel must be -1, 1, 2, 3, 4, 6 or 10");
         if (M < 0 || N < 1 || K < 1 || K > mf::kI8MaxK || M > mf::kI8MaxRows || N > mf::kI8MaxRows)
             throw std::runtime_error(std::string(who) + ": bad sizes (0 <= M, 1 <= N, both <= 2^30, 1 <= K <= 131071)");

@@ -41,6 +41,12 @@ def test_gemm_refusals(lib, reason, change):
     refused(lib.cudanet_k_gemm_i8, args, GEMM, reason, **change)
 
 
+@pytest.mark.parametrize("kernel", [0, 5, 11, 63, 65, 66, 69, 75, 128, -2, 2 ** 31 - 1, -2 ** 31])
+def test_gemm_refuses_other_kernels(lib, kernel):
+    args = (1, 0, -1, P, P, P, P, P, P, 5, 32, 64, 64, 64, 32)
+    refused(lib.cudanet_k_gemm_i8, args, GEMM, "kernel", kernel=kernel)
+
+
 NORM = ("x_type", "delta_type", "x", "delta", "g", "out", "q", "scale", "M", "D", "ldx", "ldd", "ldo", "ldq", "eps")
 
 

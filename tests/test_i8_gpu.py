@@ -327,6 +327,23 @@ def test_gelu_of_every_size(k, out):
         assert (C >= (v - e).to(C.dtype)).all() and (C <= (v + e).to(C.dtype)).all(), kernel
 
 
+@pytest.mark.parametrize("epi,out", [(1, "bf16"), (2, "f32"), (3, "f32")])
+@pytest.mark.parametrize("split", [1, 2, 8])
+def test_gemm_gives_up_without_storing(k, split, epi, out):
+    """The last CTA of each cluster is given no operands: its waits run out after 2 s, the check says so, and nothing of
+    the product is stored. The calls after it are as ever."""
+    A, W, rs, cs, bias = operands(19, 300, 2100, 11)
+    C, full = matrix(19, 300, DT[out], 304, 7)
+    C0 = C.fill_(5).clone()
+    k.k_gemm_i8(A, W, rs, cs, bias, C, epi, 64 + 2 + split)
+    with pytest.raises(RuntimeError, match="device error"):
+        k.k_i8_check()
+    assert torch.equal(C, C0) and untouched(C, full, 7)
+    k.k_gemm_i8(A, W, rs, cs, bias, C, epi, 2 + split)
+    k.k_i8_check()
+    check_product(C, C0, A, W, rs, cs, bias, epi)
+
+
 def test_gemm_offset_vectors(k):
     """Scales and bias that begin on 4 bytes, and operands that are rows of larger matrices."""
     A, W, rs, cs, bias = operands(400, 520, 256, 9)
