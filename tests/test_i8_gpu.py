@@ -282,6 +282,51 @@ def test_gemm(k, M, N, K, epi, out):
     k.k_i8_check()
 
 
+# Several tiles of 256 x 256 for each of the pair kernel's CTA pairs (74 on a GPU of 148 SMs): A's blocks kept over a row
+# of tiles (K <= 1,024) or both operands streamed, rows of tiles that end inside a pair's share, one tile a row, one row.
+PAIR_SIZES = [(9000, 1104, K) for K in (100, 128, 129, 300, 512, 640, 700, 800, 1000, 1024, 1025, 1300, 2048, 4100)] + [
+    (8500, 2060, 1000), (40000, 40, 200), (57000, 250, 300), (600, 20000, 130), (250, 60000, 1000), (1, 70000, 1040),
+    (33024, 512, 64), (20000, 1001, 1111)]
+
+
+@pytest.mark.parametrize("M,N,K", PAIR_SIZES)
+@pytest.mark.parametrize("epi,out", [(0, "bf16"), (0, "f16"), (1, "bf16"), (1, "f16"), (2, "f32"), (3, "f32")])
+def test_gemm_many_tiles_a_pair(k, M, N, K, epi, out):
+    A, W, rs, cs, bias = operands(M, N, K, M + N * 3 + K * 5 + epi)
+    if K % 2:
+        bias = None
+    first = None
+    for pitch, off in (((N + 7) // 8 * 8, 0), (N + 3, 1)):     # stored by TMA where N suits it, and by the warps
+        C, full = matrix(M, N, DT[out], pitch, 7, off)
+        if epi == 2:
+            C.copy_(torch.randn(M, N, device="cuda", generator=gen(N)))
+        C0 = C.clone()
+        for kernel in (1, 2, -1, 1):
+            C.copy_(C0)
+            k.k_gemm_i8(A, W, rs, cs, bias, C, epi, kernel)
+            if first is None:
+                check_product(C, C0, A, W, rs, cs, bias, epi)
+                first = C.clone()
+            assert torch.equal(C, first), f"kernel {kernel}, pitch {pitch}"
+        assert untouched(C, full, 7, off)
+    k.k_i8_check()
+
+
+@pytest.mark.parametrize("epi,pitch", [(0, 32768), (2, 32768), (3, 32769), (1, 32769)])
+def test_pair_offsets_past_32_bits(k, epi, pitch):
+    """The pair kernel's rows of A and C more than 2^31 elements into their buffers."""
+    M, D, N = 70000, 48, 600
+    r = gen(epi)
+    q = torch.empty(M, 32768, dtype=torch.int8, device="cuda")[:, 32768 - D:]
+    q.copy_(torch.randint(-128, 128, (M, D), device="cuda", generator=r, dtype=torch.int32).to(torch.int8))
+    W = torch.randint(-128, 128, (N, D), device="cuda", generator=r, dtype=torch.int32).to(torch.int8)
+    rs, cs = torch.rand(M, device="cuda", generator=r) + 0.5, torch.rand(N, device="cuda", generator=r) / 1000
+    C = torch.zeros(M, pitch, dtype=torch.float32 if epi >= 2 else torch.bfloat16, device="cuda")[:, :N]
+    k.k_gemm_i8(q, W, rs, cs, None, C, epi, 1)
+    check_product(C, torch.zeros(M, N, device="cuda"), q, W, rs, cs, None, epi)
+    k.k_i8_check()
+
+
 @pytest.mark.parametrize("M", [1, 20, 300])
 def test_gemm_largest_sums(k, M):
     """The longest K at the largest products: the int32 sum comes to 2^31 - 16,384."""
