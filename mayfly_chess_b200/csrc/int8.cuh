@@ -370,9 +370,11 @@ __device__ __forceinline__ void i8_pair_epilogue(const CUtensorMap* tmC, const I
         float* sv = svec + (it & 1) * 2 * COLS;              // the other half is still read by this group's slower warps
         sv[gtid] = next;
         const uint64_t rs2 = pk2(next_rs, next_rs);
-        if (gtid == 0) epi_ok[grp] = mbar_wait(&tfull[acc], acc_phase, err, kErrTmemFull) ? 1u : 0u;
+        // the group's one decision; the word of the tile before may still be read by its slower warps
+        volatile uint32_t* const go = epi_ok + (it & 1) * C::GROUPS + grp;
+        if (gtid == 0) *go = mbar_wait(&tfull[acc], acc_phase, err, kErrTmemFull) ? 1u : 0u;
         named_barrier(1 + grp, 128);
-        if (!epi_ok[grp]) break;
+        if (!*go) break;
         tc_fence_after();
         read_ahead(it + 1);
         const uint32_t t_acc = t_lane + static_cast<uint32_t>(acc * 256);
@@ -479,7 +481,7 @@ gemm_i8_pair_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_consta
     uint64_t* const tempty = tfull + 2;
     uint64_t* const mma_done = tempty + 2;
     uint32_t* const tmem_slot = reinterpret_cast<uint32_t*>(mma_done + 1);
-    volatile uint32_t* const epi_ok = tmem_slot + 1;
+    volatile uint32_t* const epi_ok = tmem_slot + 1;   // [2][GROUPS]
 
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     const uint32_t rank = cluster_ctarank();
