@@ -59,9 +59,14 @@ struct RowsI8 {
 };
 
 // 8 elements as they lie in memory, so that all of a thread's loads are on their way before the first is converted.
+// RO: nothing writes them while the kernel runs (the read-only path).
 template <typename T> struct Raw8 {
     uint4 w;
-    __device__ __forceinline__ void load(const T* p) { w = __ldg(reinterpret_cast<const uint4*>(p)); }   // on 16 bytes
+    template <bool RO> __device__ __forceinline__ void load(const T* p)   // on 16 bytes
+    {
+        const uint4* u = reinterpret_cast<const uint4*>(p);
+        w = RO ? __ldg(u) : *u;
+    }
     __device__ __forceinline__ void zero() { w = make_uint4(0, 0, 0, 0); }
     __device__ __forceinline__ void get(float (&v)[8]) const
     {
@@ -79,10 +84,11 @@ template <typename T> struct Raw8 {
 };
 template <> struct Raw8<float> {
     float4 a, b;
-    __device__ __forceinline__ void load(const float* p)
+    template <bool RO> __device__ __forceinline__ void load(const float* p)
     {
-        a = __ldg(reinterpret_cast<const float4*>(p));
-        b = __ldg(reinterpret_cast<const float4*>(p) + 1);
+        const float4* u = reinterpret_cast<const float4*>(p);
+        a = RO ? __ldg(u) : u[0];
+        b = RO ? __ldg(u + 1) : u[1];
     }
     __device__ __forceinline__ void zero() { a = b = make_float4(0.f, 0.f, 0.f, 0.f); }
     __device__ __forceinline__ void get(float (&v)[8]) const
@@ -151,8 +157,9 @@ __global__ void __launch_bounds__(L ? 128 : 1024) rows_i8_kernel(const RowsI8 a)
     const int e0 = VEC ? 8 * t : L ? t : (t >> 5) * 256 * V + (t & 31);
     const int left = D - e0;
     auto at = [&](int v, int j) { return VEC ? 8 * T * v + j : (L ? L : 32) * (8 * v + j); };
-    const XT* __restrict__ x = static_cast<const XT*>(a.x) + row * a.ldx + e0;
-    const DT* __restrict__ delta = static_cast<const DT*>(a.delta) + row * a.ldd + e0;
+    // the norm's out may be x or delta: ordinary loads, all of a thread's ahead of its first store
+    const XT* x = static_cast<const XT*>(a.x) + row * a.ldx + e0;
+    const DT* delta = static_cast<const DT*>(a.delta) + row * a.ldd + e0;
     const float* __restrict__ gp = NORM ? a.g + e0 : nullptr;
     XT* out = static_cast<XT*>(a.out) + row * a.ldo + e0;
     int8_t* q = a.q + row * a.ldq + e0;
@@ -165,13 +172,13 @@ __global__ void __launch_bounds__(L ? 128 : 1024) rows_i8_kernel(const RowsI8 a)
 #pragma unroll
         for (int v = 0; v < V; ++v) {
             rx[v].zero();
-            if (at(v, 0) < left) rx[v].load(x + at(v, 0));
+            if (at(v, 0) < left) rx[v].template load<!NORM>(x + at(v, 0));
         }
         if (add) {
 #pragma unroll
             for (int v = 0; v < V; ++v) {
                 rd[v].zero();
-                if (at(v, 0) < left) rd[v].load(delta + at(v, 0));
+                if (at(v, 0) < left) rd[v].template load<false>(delta + at(v, 0));
             }
         }
 #pragma unroll
@@ -226,7 +233,7 @@ __global__ void __launch_bounds__(L ? 128 : 1024) rows_i8_kernel(const RowsI8 a)
             if constexpr (VEC) {
                 Raw8<float> rg;
                 rg.zero();
-                if (at(v, 0) < left) rg.load(gp + at(v, 0));
+                if (at(v, 0) < left) rg.template load<true>(gp + at(v, 0));
                 rg.get(g);
             } else {
 #pragma unroll

@@ -142,6 +142,31 @@ def test_rows_of_any_pitch_and_start(k, x, D, px, pd, po, pq, off):
     assert untouched(qq, fq, 99, off)
 
 
+@pytest.mark.parametrize("x", ["f32", "bf16", "f16"])
+@pytest.mark.parametrize("M,D,pitch,off", [(3000, 1024, 1024, 0), (3000, 72, 80, 0), (2500, 727, 727, 1), (4000, 37, 37, 0),
+                                           (700, 4001, 4001, 3), (600, 8192, 8192, 0), (100, 20000, 20000, 0)])
+def test_sum_in_place(k, x, M, D, pitch, off):
+    """The sum stored over x and over delta, where rows share 32-byte sectors with their neighbours too: the bits of the
+    call that stores it elsewhere."""
+    r = gen(M + D)
+    X0 = torch.randn(M, D, device="cuda", generator=r).to(DT[x])
+    D0 = torch.randn(M, D, device="cuda", generator=r).to(DT[x])
+    G = 1 + 0.1 * torch.randn(D, device="cuda", generator=r)
+    (X, fx), (Dl, fd), (out, _) = (matrix(M, D, DT[x], pitch, 9, off) for _ in range(3))
+    X.copy_(X0)
+    Dl.copy_(D0)
+    q, scale = torch.empty(M, D, dtype=torch.int8, device="cuda"), torch.empty(M, device="cuda")
+    k.k_rmsnorm_i8(X, Dl, G, out, q, scale)
+    assert torch.equal(out, (X0.float() + D0.float()).to(DT[x])) and torch.equal(X, X0) and torch.equal(Dl, D0)
+    for place, full in ((X, fx), (Dl, fd)):
+        q2, scale2 = torch.empty_like(q), torch.empty_like(scale)
+        X.copy_(X0)
+        Dl.copy_(D0)
+        k.k_rmsnorm_i8(X, Dl, G, place, q2, scale2)
+        assert torch.equal(place, out) and torch.equal(q2, q) and torch.equal(scale2, scale)
+        assert untouched(place, full, 9, off)
+
+
 @pytest.mark.parametrize("D", [1, 33, 1024, 9000])
 @pytest.mark.parametrize("x", ["f32", "bf16", "f16"])
 def test_rows_with_nothing_to_scale(k, D, x):
