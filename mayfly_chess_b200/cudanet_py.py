@@ -660,6 +660,13 @@ def _i8_vector(once, t, name, n, dev):
         raise ValueError(f"{name}: on {t.device}, expected a tensor of one CUDA device with the others")
 
 
+def _i8_ints(**values):
+    """Raises unless each fits the C ABI's 32-bit int: ctypes would pass its low 32 bits on."""
+    for name, v in values.items():
+        if not -2 ** 31 <= v < 2 ** 31:
+            raise ValueError(f"{name}: {v} is over the 32 bits of the library's sizes")
+
+
 def k_rmsnorm_i8(x, delta, g, out, q, scale, eps=1e-6, dll=None):
     """out = x + delta in x's type, and its RMS norm times g as int8 rows with a float32 scale each: q * scale stands
     for out / sqrt(mean(out^2) + eps) * g. x (M, D) float32, bfloat16 or float16; delta the same shape, of x's type or
@@ -671,7 +678,7 @@ def k_rmsnorm_i8(x, delta, g, out, q, scale, eps=1e-6, dll=None):
     if len(shape) != 2:
         _i8_matrix(x, "x", shape, dev)
     (M, D), xs, qs = shape, x.stride(), q.stride()
-    if (dev < 0 or xs[1] != 1 or q.dtype is not once.int8 or q.shape != shape or qs[1] != 1 or q.get_device() != dev
+    if (dev < 0 or M + D >= 2 ** 31 or xs[1] != 1 or q.dtype is not once.int8 or q.shape != shape or qs[1] != 1 or q.get_device() != dev
             or g.dtype is not f32 or g.shape != (D,) or g.get_device() != dev or not g.is_contiguous()
             or scale.dtype is not f32 or scale.shape != (M,) or scale.get_device() != dev
             or not scale.is_contiguous()):
@@ -679,6 +686,7 @@ def k_rmsnorm_i8(x, delta, g, out, q, scale, eps=1e-6, dll=None):
         _i8_matrix(q, "q", shape, dev, once.int8)
         _i8_vector(once, g, "g", D, dev)
         _i8_vector(once, scale, "scale", M, dev)
+        _i8_ints(M=M, D=D)
     if delta is None:
         if out is not None:
             raise ValueError("out without delta: there is no sum to store")
@@ -713,12 +721,13 @@ def k_quant_i8(x, q, scale, dll=None):
     if len(shape) != 2:
         _i8_matrix(x, "x", shape, dev)
     (M, D), xs, qs = shape, x.stride(), q.stride()
-    if (dev < 0 or xs[1] != 1 or q.dtype is not once.int8 or q.shape != shape or qs[1] != 1 or q.get_device() != dev
+    if (dev < 0 or M + D >= 2 ** 31 or xs[1] != 1 or q.dtype is not once.int8 or q.shape != shape or qs[1] != 1 or q.get_device() != dev
             or scale.dtype is not once.f32 or scale.shape != (M,) or scale.get_device() != dev
             or not scale.is_contiguous()):
         _i8_matrix(x, "x", shape, dev)
         _i8_matrix(q, "q", shape, dev, once.int8)
         _i8_vector(once, scale, "scale", M, dev)
+        _i8_ints(M=M, D=D)
     if once.device() != dev:
         with once.on_device(dev):
             return k_quant_i8(x, q, scale, dll)
@@ -743,7 +752,7 @@ def k_gemm_i8(A, W, rowscale, colscale, bias, C, epi, kernel=-1, dll=None):
     M, K = sa
     N = sw[0]
     ta, tw, tc = A.stride(), W.stride(), C.stride()
-    if (dev < 0 or A.dtype is not i8 or ta[1] != 1 or W.dtype is not i8 or tw[1] != 1 or W.get_device() != dev
+    if (dev < 0 or M + N + K >= 2 ** 31 or (epi | kernel + 1) >> 7 or A.dtype is not i8 or ta[1] != 1 or W.dtype is not i8 or tw[1] != 1 or W.get_device() != dev
             or C.shape != (M, N) or tc[1] != 1 or C.get_device() != dev or rowscale.dtype is not f32
             or rowscale.shape != (M,) or rowscale.get_device() != dev or not rowscale.is_contiguous()
             or colscale.dtype is not f32 or colscale.shape != (N,) or colscale.get_device() != dev
@@ -753,6 +762,7 @@ def k_gemm_i8(A, W, rowscale, colscale, bias, C, epi, kernel=-1, dll=None):
         _i8_matrix(C, "C", (M, N), dev)
         _i8_vector(once, rowscale, "rowscale", M, dev)
         _i8_vector(once, colscale, "colscale", N, dev)
+        _i8_ints(M=M, N=N, K=K, epi=epi, kernel=kernel)
     bp = None
     if bias is not None:
         if (bias.dtype is not f32 or bias.shape != (N,) or bias.get_device() != dev or not bias.is_contiguous()):

@@ -93,3 +93,84 @@ def test_wrappers_refuse_host_tensors():
         k.k_rmsnorm_i8(x, x, torch.ones(16), x, q, s)
     with pytest.raises(ValueError, match="CUDA"):
         k.k_gemm_i8(q, q, s, s, None, torch.empty(2, 2), 3)
+
+
+class Fake:
+    """What the wrappers ask of a tensor on device 0, without its memory."""
+
+    def __init__(self, dtype, *shape):
+        import torch
+        self.dtype, self.shape, self.device = dtype, torch.Size(shape), "cuda:0"
+
+    def stride(self, i=None):
+        st = [1]
+        for n in self.shape[:0:-1]:
+            st.insert(0, st[0] * n)
+        return tuple(st) if i is None else st[i]
+
+    def get_device(self):
+        return 0
+
+    def is_contiguous(self):
+        return True
+
+    def data_ptr(self):
+        return P
+
+
+@pytest.fixture
+def calls(monkeypatch):
+    """The wrappers with a library that notes its calls in place of the real one."""
+    from mayfly_chess_b200 import cudanet_py as k
+    seen = []
+
+    class Lib:
+        def __getattr__(self, name):
+            return lambda *args: seen.append((name, args)) or 0
+    once = k._I8Once()
+    once.device, once.stream, once.lib = (lambda: 0), (lambda dev: 0), Lib()
+    monkeypatch.setattr(k, "_i8_once", once)
+    return k, seen
+
+
+BIG = 2 ** 32 + 32   # its low 32 bits are a size like any other
+
+
+@pytest.mark.parametrize("M,D", [(BIG, 64), (4, BIG), (2 ** 31, 64), (BIG, BIG)])
+def test_wrappers_refuse_rows_over_32_bits(calls, M, D):
+    import torch
+    k, seen = calls
+    f32 = torch.float32
+    x, q, g, s = Fake(f32, M, D), Fake(torch.int8, M, D), Fake(f32, D), Fake(f32, M)
+    with pytest.raises(ValueError, match="32 bits"):
+        k.k_quant_i8(x, q, s)
+    with pytest.raises(ValueError, match="32 bits"):
+        k.k_rmsnorm_i8(x, x, g, x, q, s)
+    assert not seen
+
+
+@pytest.mark.parametrize("change", [{"M": BIG}, {"N": BIG}, {"K": BIG}, {"epi": 2 ** 32 + 2}, {"kernel": 2 ** 32 + 1},
+                                    {"kernel": 2 ** 32 - 1}, {"epi": 2 ** 31, "kernel": -2 ** 31 - 1}])
+def test_gemm_wrapper_refuses_numbers_over_32_bits(calls, change):
+    import torch
+    k, seen = calls
+    v = {"M": 4, "N": 32, "K": 64, "epi": 3, "kernel": -1, **change}
+    i8, f32 = torch.int8, torch.float32
+    with pytest.raises(ValueError, match="32 bits"):
+        k.k_gemm_i8(Fake(i8, v["M"], v["K"]), Fake(i8, v["N"], v["K"]), Fake(f32, v["M"]), Fake(f32, v["N"]), None,
+                    Fake(f32, v["M"], v["N"]), v["epi"], v["kernel"])
+    assert not seen
+
+
+def test_wrappers_pass_what_they_are_given(calls):
+    """The same stand-ins with sizes in range reach the library, so the refusals above are of the sizes."""
+    import torch
+    k, seen = calls
+    i8, f32 = torch.int8, torch.float32
+    x, q, g, s = Fake(f32, 5, 64), Fake(i8, 5, 64), Fake(f32, 64), Fake(f32, 5)
+    k.k_quant_i8(x, q, s)
+    k.k_rmsnorm_i8(x, x, g, x, q, s)
+    k.k_gemm_i8(q, Fake(i8, 32, 64), s, Fake(f32, 32), None, Fake(f32, 5, 32), 3, 10)
+    k.k_gemm_i8(q, Fake(i8, 32, 64), s, Fake(f32, 32), None, Fake(f32, 5, 32), 4, -2)     # the library's to refuse
+    assert [n for n, _ in seen] == ["cudanet_k_quant_i8", "cudanet_k_rmsnorm_i8"] + ["cudanet_k_gemm_i8"] * 2
+    assert seen[2][1][9:12] == (5, 32, 64) and seen[3][1][1:3] == (4, -2)
