@@ -781,9 +781,11 @@ def k_gemm_i8(A, W, rowscale, colscale, bias, C, epi, kernel=-1, dll=None):
 
 def k_i8_check(stream=None, dll=None):
     """Wait for `stream` (a torch.cuda.Stream, default the current one) and raise if a bounded wait of a k_gemm_i8 call
-    on the current device has failed since the last check."""
+    on its device has failed since the last check."""
     import torch
     s = stream if stream is not None else torch.cuda.current_stream()
     err = ctypes.create_string_buffer(ERR_LEN)
-    if load(dll).cudanet_k_i8_check(ctypes.c_void_p(s.cuda_stream), err, ERR_LEN) != 0:
+    with torch.cuda.device(s.device):
+        rc = load(dll).cudanet_k_i8_check(ctypes.c_void_p(s.cuda_stream), err, ERR_LEN)
+    if rc != 0:
         raise RuntimeError(f"cudanet_k_i8_check: {_msg(err)}")

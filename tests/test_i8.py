@@ -174,3 +174,32 @@ def test_wrappers_pass_what_they_are_given(calls):
     k.k_gemm_i8(q, Fake(i8, 32, 64), s, Fake(f32, 32), None, Fake(f32, 5, 32), 4, -2)     # the library's to refuse
     assert [n for n, _ in seen] == ["cudanet_k_quant_i8", "cudanet_k_rmsnorm_i8"] + ["cudanet_k_gemm_i8"] * 2
     assert seen[2][1][9:12] == (5, 32, 64) and seen[3][1][1:3] == (4, -2)
+
+
+def test_check_asks_the_streams_device(monkeypatch):
+    """The library reads the word of the current device, so the stream's has to be it while the library is called."""
+    import contextlib
+
+    import torch
+    from mayfly_chess_b200 import cudanet_py as k
+    current, seen = [0], []
+
+    @contextlib.contextmanager
+    def device(d):
+        before, current[0] = current[0], torch.device(d).index
+        yield
+        current[0] = before
+
+    class Stream:
+        device, cuda_stream = torch.device("cuda:3"), 77
+
+    class Lib:
+        def cudanet_k_i8_check(self, stream, err, err_len):
+            seen.append((current[0], stream.value))
+            return -1 if len(seen) > 1 else 0
+    monkeypatch.setattr(torch.cuda, "device", device)
+    monkeypatch.setattr(k, "load", lambda dll=None: Lib())
+    k.k_i8_check(Stream())
+    with pytest.raises(RuntimeError):
+        k.k_i8_check(Stream())
+    assert seen == [(3, 77)] * 2 and current[0] == 0
