@@ -112,6 +112,48 @@ def test_rmsnorm(k, M, D, x, delta):
         assert torch.equal(X, want) and torch.equal(q2, q) and torch.equal(scale2, scale)
 
 
+# A width on each side of every border between two row kernels, aligned and element by element, rows that leave part of a
+# block or of a warp without one.
+WIDTHS = [(M, D, off) for M, D in ((7, 8), (7, 64), (131, 72), (13, 128), (131, 136), (5, 256), (131, 264), (6, 512), (131, 520),
+                                   (5, 768), (131, 776), (6, 1024), (131, 1032), (5, 1288), (131, 1536), (5, 1544),
+                                   (131, 2048), (3, 2056), (3, 16384), (3, 16392), (2, 32768)) for off in (0, 1)]
+WIDTHS += [(M, D, 1) for M, D in ((131, 1), (7, 65), (131, 129), (7, 257), (131, 511), (7, 513), (131, 600), (5, 767),
+                                  (131, 769), (5, 1023), (131, 1025), (5, 2047), (5, 2049), (3, 16383), (3, 16385), (2, 32767))]
+
+
+@pytest.mark.parametrize("M,D,off", WIDTHS)
+@pytest.mark.parametrize("x,delta", [("f32", "f32"), ("f32", "bf16"), ("f32", "f16"), ("f32", None), ("bf16", "bf16"),
+                                     ("bf16", None), ("f16", "f16"), ("f16", None)])
+def test_rows_of_every_width(k, M, D, off, x, delta):
+    """Codes of the norm as of test_rmsnorm. Its scale: at most 32 squares in a thread and 10 sums over warp and block,
+    42u, halved by the root; the mean and eps u together after it, rsqrtf 4u, the largest, its product and the quotient
+    u each: 29u, and 1u for products of these. Where the norm adds nothing, the quantiser of the same rows too."""
+    r = gen(M * 41 + D)
+    X, _ = matrix(M, D, DT[x], (D + 7) // 8 * 8 if off == 0 else D, 9, off)
+    X.copy_(torch.randn(M, D, device="cuda", generator=r))
+    X[:, D // 2] = 4.0
+    G = 1 + 0.1 * torch.randn(D, device="cuda", generator=r)
+    Dl = torch.randn(M, D, device="cuda", generator=r).to(DT[delta]) if delta else None
+    want = X if delta is None else (X.float() + Dl.float()).to(X.dtype)
+    out = torch.empty(M, D, dtype=X.dtype, device="cuda") if delta else None
+    q, fq = matrix(M, D, torch.int8, (D + 15) // 16 * 16, 99)
+    scale = torch.full((M + 1,), 9.0, device="cuda")
+    k.k_rmsnorm_i8(X, Dl, G, out, q, scale[:M], 1e-5)
+    if delta:
+        assert torch.equal(out, want)
+    s = want.double()
+    t = (want.float() * G).double()
+    scale64 = (s * G.double()).abs().amax(1) / torch.sqrt(s.square().mean(1) + float(torch.tensor(1e-5))) / 127
+    check_codes(q, scale[:M], s * G.double(), scale64, 30 * U)
+    assert torch.equal(q.float(), torch.round((127 * t / t.abs().amax(1, keepdim=True)).float()))
+    assert untouched(q, fq, 99) and scale[M] == 9
+    if delta is None:
+        k.k_quant_i8(X, q, scale[:M])
+        assert torch.equal(scale[:M], row_scale(X))
+        assert torch.equal(q.float(), torch.round((127 * s / s.abs().amax(1, keepdim=True)).float()))
+        assert untouched(q, fq, 99) and scale[M] == 9
+
+
 @pytest.mark.parametrize("x", ["f32", "bf16", "f16"])
 @pytest.mark.parametrize("D,px,pd,po,pq,off", [(64, 64, 80, 72, 64, 0), (64, 65, 66, 67, 68, 1), (1000, 1008, 1000, 1001, 1008, 0),
                                                (100, 112, 104, 108, 112, 3), (2048, 2056, 2049, 2048, 2064, 8)])
