@@ -573,6 +573,40 @@ def test_block_on_another_stream_and_replayed(k):
     del graphs
 
 
+def test_block_from_threads(k):
+    """Four host threads, each with a stream and a block of its own sizes, at the same time: the bits of one after the
+    other."""
+    import threading
+    sizes = [(1, 256, 1024), (325, 512, 1008), (2080, 1024, 2048), (9000, 256, 1104)]
+    blocks = [block_state(k, *n, 90 + i) for i, n in enumerate(sizes)]
+    names = ("out", "q", "s", "h", "q2", "s2")
+    want = []
+    for b in blocks:
+        block(k, b)
+        want.append([b[n].clone() for n in names])
+    torch.cuda.synchronize()
+    failed = []
+
+    def work(b, w):
+        try:
+            with torch.cuda.stream(torch.cuda.Stream()):
+                for _ in range(30):
+                    for n in names:
+                        b[n].zero_()
+                    block(k, b)
+                    if not all(torch.equal(b[n], t) for n, t in zip(names, w)):
+                        failed.append("other bits")
+                k.k_i8_check()
+        except Exception as e:
+            failed.append(repr(e))
+    threads = [threading.Thread(target=work, args=a) for a in zip(blocks, want)]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join()
+    assert not failed
+
+
 def test_first_call_of_a_process_captured(k):
     """Each operator's first call of a process inside a stream capture: nothing in it may need an earlier call."""
     import subprocess
