@@ -228,9 +228,9 @@ CUDANET_API int cudanet_k_quant_i8(int x_type, const void* x, void* q, float* sc
  * int32 sum (any int8 codes, -128 included; 1 <= K <= 131,071, the largest K whose sums fit; M and N up to 2^30), with
  * epi as for cudanet_k_gemm: 0: C 16-bit (`dtype`) = v; 1: C 16-bit = gelu(v); 2: C f32 += v; 3: C f32 = v. A and W begin
  * on 16 bytes and their row pitches are multiples of 16; C, bias and the scales may begin anywhere and C have any pitch
- * >= N (fastest where C's start, row and pitch are whole 16-byte units and the operands' rows begin on 128). kernel -1 chooses; 1 asks for 256 x 256 tiles on
- * CTA pairs, 2 for the kernel with weights on the tensor cores' lanes and K split as it chooses, 3, 4, 6 and 10 for that
- * with K split over 1, 2, 4 and 8 CTAs (fewer where K has fewer blocks of 128). Every kernel gives the same bits (epi 2
+ * >= N (fastest where C's start, row and pitch are whole 16-byte units and the operands' rows begin on 128). kernel -1
+ * chooses; 1 asks for 256 x 256 tiles on CTA pairs, 2 for the kernel with weights on the tensor cores' lanes and K split
+ * as it chooses, 3, 4, 6 and 10 for that with K split over 1, 2, 4 and 8 CTAs (fewer where K has fewer blocks of 128). Every kernel gives the same bits (epi 2
  * adds once an element in L2, which may take a sum below the smallest normal f32 for 0). A wait inside the kernel that runs
  * out (a failure of the device) ends it with C partly unwritten, never with a sum that lacks a part, and is reported by
  * cudanet_k_i8_check. For tests, 67, 68, 70 and 74 are 3, 4, 6 and 10 with no operands for each cluster's last CTA, whose

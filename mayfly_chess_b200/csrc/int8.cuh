@@ -286,7 +286,8 @@ __global__ void __launch_bounds__(L ? 128 : 1024) rows_i8_kernel(const RowsI8 a)
     for (int v = 0; v < V; ++v) {
         if constexpr (VEC) {
             if (at(v, 0) < left)
-                *reinterpret_cast<uint2*>(q + at(v, 0)) = make_uint2(codes4<UP, PAIRED>(s[v], rs), codes4<UP, PAIRED>(s[v] + 4, rs));
+                *reinterpret_cast<uint2*>(q + at(v, 0)) =
+                    make_uint2(codes4<UP, PAIRED>(s[v], rs), codes4<UP, PAIRED>(s[v] + 4, rs));
         } else {
 #pragma unroll
             for (int j = 0; j < 8; j += 2) {
@@ -323,10 +324,10 @@ struct I8Out {
 // fastest, and keeps its rows of A in shared memory over all of them where they fit (K <= 1,024): only W then streams.
 // What paced the products before was their issue: by one lane of a diverged warp, with two commits a stage, 187 cycles an
 // instruction; from a converged warp with one commit to both CTAs 128 to 140 (66,560 x 2,048 x 1,024: 131 -> 113 us).
-// What bounds it now: 8,192^3 keeps the tensor cores busy 92% of their cycles (2,630 TOP/s); the 1,000 W cap, which takes
-// the clock from 1.97 to about 1.4 GHz in a long run (66,560 x 2,048 x 1,024 there 134 us, with GELU 147 to 150; cool 109
-// and 122); and with GELU the epilogue's instructions (7,100 cycles a tile against 6,100 without it and 4,096 of
-// products). Roles: warp 0 TMA loads, warp 1 tensor memory and the products (leader CTA), warps 2..17 the epilogue.
+// What bounds it now: 8,192^3 keeps the tensor cores busy 92% of their cycles (2,600 TOP/s); the 1,000 W cap, which takes
+// the clock from 1.97 to about 1.4 GHz in a long run (66,560 x 2,048 x 1,024 there 133 us, with GELU 156; cool 111 and
+// 131); and with GELU the epilogue's instructions (7,900 cycles a tile, 6,100 without it, 4,096 of products).
+// Roles: warp 0 TMA loads, warp 1 tensor memory and the products (leader CTA), warps 2..17 the epilogue.
 struct I8PairCfg {
     static constexpr int SLOTS = 11;                     // of 128 rows x 128 bytes
     static constexpr uint32_t SLOT = 128 * 128;
@@ -340,8 +341,9 @@ struct I8PairCfg {
 
 // A warp owns 32 rows of the tile and COLS neighbouring columns: it converts them from tensor memory into its own
 // staging chunk, and its lane 0 stores the chunk (for the residual: adds it at L2) by TMA, so that the warps of a group
-// meet once a tile and not at every chunk; where C does not suit TMA, the warp stores the chunk row by row. The group's column scales and bias of a tile are read by its 128 threads a
-// tile ahead and passed through shared memory: each is read once from L2, and an aligned float4 serves a warp.
+// meet once a tile and not at every chunk; where C does not suit TMA, the warp stores the chunk row by row. The group's
+// column scales and bias of a tile are read by its 128 threads a tile ahead and passed through shared memory: each is
+// read once from L2, and an aligned float4 serves a warp.
 template <typename TO, int EPI, typename OriginFn, typename ReleaseFn>
 __device__ __forceinline__ void i8_pair_epilogue(const CUtensorMap* tmC, const I8Out& p, uint8_t* stages, float* vecs,
                                                  volatile uint32_t* epi_ok, uint64_t* tfull, uint32_t tmem_base,
@@ -632,14 +634,15 @@ gemm_i8_pair_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_consta
 }
 
 // ------------------------------------------------------------------------------------------------ few rows
-// The product for few rows of A. The weight takes the 128 lanes
-// of the tensor-core instruction (M = 128 rows of W) and the tokens its columns (N = TN rows of A), so that a few tokens
-// waste little and a thread of the epilogue owns an output channel: its column scale and bias stay in two registers,
-// and a warp stores 32 neighbouring channels of a row, wherever the row begins. K is split over a cluster of S CTAs,
-// which fills the GPU where the tiles alone do not: each CTA leaves its exact int32 partial sums in its shared memory
-// and sums a share of the tokens over the cluster through distributed shared memory. No workspace, no atomics. Bound by
-// what W takes from HBM plus about 5 us (start, first bytes, exchange): 16 x 32,768 x 8,192 45.6 us (5.9 TB/s), 16 x 8,192
-// x 8,192 15.2 us, out of L2 9.4 us; 1 x 8,324 x 1,024 4.3 us; 777 x 1,001 x 1,000 added in place 6.7 us (7.9 where it reads, adds and writes).
+// The product for few rows of A. The weight takes the 128 lanes of the tensor-core instruction (M = 128 rows of W) and the
+// tokens its columns (N = TN rows of A), so that a few tokens waste little and a thread of the epilogue owns an output
+// channel: its column scale and bias stay in two registers, and a warp stores 32 neighbouring channels of a row, wherever
+// the row begins. K is split over a cluster of S CTAs, which fills the GPU where the tiles alone do not: each CTA leaves
+// its exact int32 partial sums in its shared memory and sums a share of the tokens over the cluster through distributed
+// shared memory, without a workspace; where a CTA of the cluster has given up on a wait, none stores. Bound by
+// what W takes from HBM plus about 5 us (start, first bytes, exchange): 16 x 32,768 x 8,192 43.8 us (6.1 TB/s),
+// 16 x 8,192 x 8,192 15.4 us, out of L2 9.7 us; 1 x 8,324 x 1,024 4.3 us; 777 x 1,001 x 1,000 added in place 6.7 us (7.9
+// where it reads, adds and writes).
 template <int TN> struct I8SplitCfg {
     static constexpr uint32_t W_BYTES = 128 * 128, A_BYTES = TN * 128, STAGE_BYTES = W_BYTES + A_BYTES;
     static constexpr int STAGES = TN == 128 ? 3 : TN == 64 ? 4 : 5;   // two CTAs an SM
@@ -803,8 +806,8 @@ gemm_i8_split_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_const
         // this CTA's share of the tokens, its groups' tokens neighbouring pairs
         const int ta = static_cast<int>(tokens * rank / S), tb = static_cast<int>(tokens * (rank + 1) / S);
         if (warp >= 2) {
-            // A sum that lacks a CTA's part is not stored: lane r reads whether CTA r's is there, the sums' own loads under
-            // way (16 x 8,192 x 8,192 9.62 us, 9.54 without; every lane reading all words before them 9.84).
+            // A sum that lacks a CTA's part is not stored: lane r reads whether CTA r's is there, the sums' own loads
+            // under way (16 x 8,192 x 8,192 9.62 us, 9.54 without; every lane reading all words before them 9.84).
             const uint32_t there = lane < static_cast<int>(S) ? ld_cluster(mapa_shared(smem_u32(s_ok), lane)) : 1u;
             const uint32_t mine = smem_u32(part) + 4u * static_cast<uint32_t>(n_in);
             for (int t = ta + 2 * grp; t < tb; t += 2 * C::GROUPS) {

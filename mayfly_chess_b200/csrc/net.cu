@@ -1682,7 +1682,7 @@ static void launch_rows_i8_cfg(const RowsI8& a, int num_sms, cudaStream_t s)
     int rows = 1, threads = (a.D + 8 * V - 1) / (8 * V);   // a block a row
     if (L) {
         // part of a warp a row: 128 threads a block, fewer while that leaves SMs without one (16,640 x 1,024 bf16 norm:
-        // 21.5 us, 24.1 with 256 threads; 66,560 x 256 f32 + bf16: 29.3 us, 35.4 with 64)
+        // 21.8 us, 24.5 with 256 threads; 66,560 x 256 f32 + bf16: 29.3 us, 34.7 with 64)
         const int warps = (a.M + 32 / (L ? L : 32) - 1) / (32 / (L ? L : 32));
         threads = 32 * std::clamp(warps / num_sms, 1, 4);
         rows = threads / (L ? L : 32);
@@ -1692,11 +1692,13 @@ static void launch_rows_i8_cfg(const RowsI8& a, int num_sms, cudaStream_t s)
 }
 
 // Part of a warp up to 1,024 elements (2,048 for the 16-bit quantiser), then a block a row: as few threads as hold the
-// row with enough loads on their way. Measured (GB/s, 66,560 x 2,048 bf16 quantised: a warp of 8 vectors a thread 6,946,
-// a block of 2 5,843; 4,097 x 8,192 bf16 norm: blocks of 4 vectors 6,138, of 2 5,312, of 1 4,327). Element by
-// element: 20,871 x 727 f16 quantised in a warp 4,018, a block a row about half of that; 16,000 x 4,001 f16 norm in blocks
-// of 16 elements a thread 4,626, of 8 4,297, of 32 3,989, the quantiser there 4,407, 3,557 and 4,661, but 8,000 x 1,301
-// 3,141, 2,799 and 2,735; 45,120 x 70 bf16 norm in half a warp a row 2,202, in a warp 1,375.
+// row with enough loads on their way. Measured (GB/s, 66,560 x 2,048 bf16 quantised: a warp of 8 vectors a thread 6,990,
+// a block of 2 5,800; 4,097 x 8,192 bf16 norm: blocks of 4 vectors 5,870, of 2 4,980, of 1 4,770). Element by
+// element: 20,871 x 727 f16 quantised in a warp 3,810, a block a row 2,050; 16,000 x 4,001 f16 norm in blocks of 16
+// elements a thread 4,520, of 8 4,170, of 32 3,900, the quantiser there 4,230, 3,460 and 4,370, but 8,000 x 1,301
+// quantised 2,970, of 8 2,620; 45,120 x 70 bf16 norm in half a warp a row 2,140, in a warp 1,290. The norm's blocks of 4
+// vectors (or 32 elements) a thread and the quantiser's of 8 are held to 64 registers by the bound of 1,024 threads and
+// spill 28 to 160 bytes a thread.
 template <typename XT, typename DT, bool NORM>
 static void launch_rows_i8_t(const RowsI8& a, int num_sms, cudaStream_t s)
 {

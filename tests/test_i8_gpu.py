@@ -11,6 +11,9 @@ Tolerances count the roundings between the definition and the result, u = 2^-24 
            result, and twice that bounds them; the 16-bit output adds eps / 2 of its type, GELU the relative
            error of Phi(-a) of its polynomial (2.5e-5 for f16, 2.6e-4 for bf16) times a * Phi(-a), which is at most
            0.17, and its slope of at most 1.13
+These bounds of the codes and of the bf16 GELU are wider than what the kernels hold: test_codes_are_the_rounded_quotient,
+test_rows_of_every_width (which counts the squares that a thread adds by its elements) and test_gelu_of_every_size have
+their own.
 """
 import math
 
