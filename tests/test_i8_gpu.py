@@ -115,6 +115,23 @@ def test_rmsnorm(k, M, D, x, delta):
         assert torch.equal(X, want) and torch.equal(q2, q) and torch.equal(scale2, scale)
 
 
+@pytest.mark.parametrize("D,off", [(64, 0), (2048, 0), (999, 1)])
+@pytest.mark.parametrize("x,low,high", [("f32", -119, 125), ("bf16", -119, 125), ("f16", -20, 13)])
+def test_codes_at_the_ends_of_the_range(k, x, low, high, D, off):
+    """Rows whose largest comes near the least that is scaled (or f16's least) and near the type's greatest."""
+    e = torch.arange(low, high + 1, device="cuda")
+    r = gen(D)
+    base = torch.randn(len(e), D, device="cuda", generator=r).clamp(-3.9, 3.9)
+    base[:, 1], base[:, D - 1] = 2.0, -1.0
+    X, _ = matrix(len(e), D, DT[x], D, 0, off)
+    X.copy_(torch.ldexp(base.to(DT[x]).double(), e[:, None]))
+    q, scale = torch.empty(len(e), D, dtype=torch.int8, device="cuda"), torch.empty(len(e), device="cuda")
+    k.k_quant_i8(X, q, scale)
+    t = X.double()
+    assert torch.equal(scale, row_scale(X)) and (scale > 0).all()
+    assert torch.equal(q.float(), torch.round((127 * t / t.abs().amax(1, keepdim=True)).float()))
+
+
 # A width on each side of every border between two row kernels, aligned and element by element, rows that leave part of a
 # block or of a warp without one.
 WIDTHS = [(M, D, off) for M, D in ((7, 8), (7, 64), (131, 72), (13, 128), (131, 136), (5, 256), (131, 264), (6, 512), (131, 520),
